@@ -55,6 +55,8 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--float32-weights", choices=["keep", "round", "refuse"], default="keep",
                    help="matrices stored in 32-bit under --dtype bfloat16: keep them (slow, announced), "
                         "round them to bfloat16 at load, or refuse the checkpoint")
+    g.add_argument("--kv-dtype", choices=["auto", "fp8"], default=None,
+                   help="keys and values in the cache: as --dtype, or in 8 bits with a scale to a row")
     g.add_argument("--page-tokens", "--page-size", dest="page_tokens", type=int, help="tokens per cache page")
     g.add_argument("--chunk-tokens", "--prefill-chunk", dest="chunk_tokens", type=int,
                    help="largest portion of one prompt per step")
@@ -123,6 +125,7 @@ def cmd_generate(args) -> int:
     if not model_path:
         raise SystemExit("allpaca generate: give --model DIR or --synthetic [PRESET]")
     llm = LLM(model=model_path, dtype=args.dtype or "auto", seed=seed, float32_weights=args.float32_weights,
+              kv_dtype=pick(args.kv_dtype, sec("kv").get("dtype", "auto")),
               page_size=pick(args.page_tokens, sec("kv").get("page_tokens", 16)),
               prefill_chunk=pick(args.chunk_tokens, sec("prefill").get("chunk_tokens", 512)),
               max_num_seqs=pick(args.max_active_requests, sec("engine").get("max_active_requests", 64)),

@@ -29,6 +29,13 @@ def parse_dtype(name) -> torch.dtype:
         raise ConfigError(f"dtype {name!r} is not supported (bfloat16, float32)") from None
 
 
+def parse_kv_dtype(name) -> str:
+    key = str(name if name is not None else "auto").lower().replace("torch.", "")
+    if key in ("auto", "fp8", "fp8_e4m3", "float8_e4m3fn"):
+        return "auto" if key == "auto" else "fp8"
+    raise ConfigError(f"kv_dtype {name!r} is not supported (auto, fp8)")
+
+
 @dataclass
 class EngineConfig:
     dtype: torch.dtype = torch.bfloat16
@@ -43,6 +50,7 @@ class EngineConfig:
     seed: int = 0xA110ACA                   # crates/allpaca-core/src/sampling.rs:6
     use_cuda_graphs: bool = True
     device: str = "cuda:0"
+    kv_dtype: str = "auto"                  # keys and values in the cache: auto (as dtype) | fp8 (8 bits, a scale to a row)
     float32_weights: str = "keep"           # matrices stored in 32-bit under a bfloat16 engine: keep | round | refuse
 
     def validate(self) -> None:
@@ -54,6 +62,7 @@ class EngineConfig:
             raise ConfigError("num_pages must be positive")
         if not (0.0 < self.gpu_memory_fraction <= 1.0):
             raise ConfigError("gpu_memory_fraction must be in (0, 1]")
+        self.kv_dtype = parse_kv_dtype(self.kv_dtype)
         if self.float32_weights not in ("keep", "round", "refuse"):
             raise ConfigError(f"float32_weights must be keep, round or refuse, not {self.float32_weights!r}")
         if self.max_num_batched_tokens < self.max_num_seqs:

@@ -52,11 +52,13 @@ class LLM:
                  max_cache_tokens: Optional[int] = None, max_num_seqs: int = 64,
                  max_num_batched_tokens: int = 2048, prefill_chunk: int = 512,
                  max_model_len: Optional[int] = None, gpu_memory_fraction: float = 0.85,
-                 device: str = "cuda:0", float32_weights: str = "keep",
+                 device: str = "cuda:0", float32_weights: str = "keep", kv_dtype: str = "auto",
                  runner: Optional[ModelRunner] = None, sampler=None):
         """``dtype``: ``"bfloat16"``, ``"float32"`` or ``"auto"`` (what the model folder's
         config.json names as ``torch_dtype``).  ``float32_weights``: what a bfloat16 engine does
-        with matrices stored in 32-bit (``"keep"`` and say so, ``"round"``, ``"refuse"``)."""
+        with matrices stored in 32-bit (``"keep"`` and say so, ``"round"``, ``"refuse"``).
+        ``kv_dtype``: how the cache keeps keys and values, ``"auto"`` (as ``dtype``) or ``"fp8"`` (8 bits with a scale to
+        a row: about twice the tokens in the same memory; grouped-query attention takes it)."""
         if runner is None:
             if model is None:
                 raise ValueError("LLM needs a model folder (or a ready runner)")
@@ -65,7 +67,7 @@ class LLM:
                                max_num_batched_tokens=max_num_batched_tokens,
                                prefill_chunk=prefill_chunk, max_model_len=max_model_len,
                                gpu_memory_fraction=gpu_memory_fraction, device=device,
-                               float32_weights=float32_weights)
+                               float32_weights=float32_weights, kv_dtype=kv_dtype)
             if seed is not None:
                 cfg.seed = seed
             runner = ModelRunner(model, cfg)

@@ -18,8 +18,9 @@ import torch
 
 from ..cache import CacheManager, GroupLayout, GroupStorage, StateStorage
 from ..config import EngineConfig
+from ..config.model_config import ConfigError
 from ..models import DecoderModel, load_config
-from ..parts import BuildEnv, Workspace
+from ..parts import BuildEnv, KV8Need, Workspace
 from ..weights import load_checkpoint
 from .. import ops
 from ..ops import library
@@ -43,7 +44,7 @@ class ModelRunner:
         torch.cuda.set_device(self.device)
         self.workspace = Workspace(self.device)
         self.env = BuildEnv(dtype=engine.dtype, device=self.device, workspace=self.workspace,
-                            page_size=engine.page_size, max_seqs=engine.max_num_seqs)
+                            page_size=engine.page_size, max_seqs=engine.max_num_seqs, kv_dtype=engine.kv_dtype)
         if model is None:
             arch, cfg = load_config(model_path)
             model = DecoderModel(arch.spec_builder(cfg), self.env)
@@ -72,6 +73,11 @@ class ModelRunner:
     def _setup_caches(self) -> None:
         e = self.engine
         self.cache_plan = self.model.cache_plan()
+        in8 = [isinstance(g.need, KV8Need) for g in self.cache_plan]
+        if e.kv_dtype == "fp8" and not (in8 and all(in8)):
+            raise ConfigError("kv_dtype fp8 needs a model whose caches all are keys and values of grouped-query attention")
+        if e.kv_dtype != "fp8" and any(in8):
+            raise ConfigError("the model was built to keep keys and values in 8 bits, the engine was not")
         page_bytes = [len(g.runs) * g.need.page_bytes(e.page_size, e.dtype) for g in self.cache_plan]
         if e.num_pages is not None:
             num_pages = e.num_pages

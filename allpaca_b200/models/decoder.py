@@ -18,8 +18,8 @@ from typing import Dict, List, Mapping, Optional, Tuple
 import torch
 
 from .. import ops
-from ..parts import (Block, BuildEnv, CacheNeed, Deferred, LayerCache, ModelSpec, Part, Slices, StreamUpdate,
-                     WeightSpec, build)
+from ..parts import (Block, BuildEnv, CacheNeed, Deferred, KV8Need, LayerCache, ModelSpec, Part, Slices,
+                     StreamUpdate, WeightSpec, build)
 from ..parts.linear import Linear
 
 
@@ -136,7 +136,9 @@ class DecoderModel:
         run ``r`` or None."""
         where: Dict[int, Tuple[int, int]] = {}
         # (all pages of a group, index of the page-size dimension), for the clearing of fresh pages
-        self._group_pages = [(storages[g].pages, 2 + len(grp.need.outer)) for g, grp in enumerate(plan)]
+        # (the kernels of 8-bit pages read only what was written)
+        self._group_pages = [(g, storages[g].pages, 2 + len(grp.need.outer)) for g, grp in enumerate(plan)
+                             if not isinstance(grp.need, KV8Need)]
         for g, grp in enumerate(plan):
             for i, r in enumerate(grp.runs):
                 where[r] = (g, i)
@@ -169,7 +171,7 @@ class DecoderModel:
         s = self.spec
         step.shared.clear()
         # pages that get their first token in this step: nothing of their last owner stays readable
-        for g, (pages, page_dim) in enumerate(self._group_pages):
+        for g, pages, page_dim in self._group_pages:
             ops.clear_page_tails(pages, page_dim, step.positions, step.token_seq, step.block_tables[g],
                                  step.context_lens)
         if s.streams is None:

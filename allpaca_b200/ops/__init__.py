@@ -858,3 +858,4 @@ from .routed import (gated_act, moe_combine, moe_down, moe_gate_up, moe_gather, 
                      moe_route, moe_route_rows, moe_sort)
 from .stream import add_dyt, bias_act, dyt_shift, stream_mix, stream_norm  # noqa: E402
 from .recurrent import exp_gates, gated_postnorm, gated_row_add, head_norm_gate, linear_scan  # noqa: E402
+from .kv8 import attention_kv8, kv8_page_bytes, kv8_read, rope_kv8_store  # noqa: E402

@@ -1,0 +1,148 @@
+"""Python faces of the kernels of the 8-bit cache of keys and values; see ``ops/__init__.py``.
+
+A page holds, for every KV head, ``page_size`` rows of ``head_dim`` e4m3 numbers for the keys and as many for the values, then one
+scale byte to a row: its values are the numbers times ``2^(byte - 127)``, the smallest power of two between 2^-60 and 2^40 under
+which no number of the row exceeds 448.  Pages are flat: ``cache_layer`` is uint8 ``[pages, kv8_page_bytes(...)]``, numbers
+``[2, kv_heads, page_size, head_dim]`` then scales ``[2, kv_heads, page_size]``.  What no row was written to is never read.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from . import AP_BF16, AP_F32, KernelError, call, core, library, stream_handle
+
+_CODES = {torch.float32: AP_F32, torch.bfloat16: AP_BF16}
+
+
+def kv8_page_bytes(num_kv_heads: int, page_size: int, head_dim: int) -> int:
+    """Bytes of one page of one layer's 8-bit cache (numbers, scales, padding to 16)."""
+    return -(-2 * num_kv_heads * page_size * (head_dim + 1) // 16) * 16
+
+
+def _take(what: str, t: torch.Tensor, name: str, dtype, dims: int, device: int) -> None:
+    if t.dtype is not dtype or t.dim() != dims or t.get_device() != device or not t.is_contiguous():
+        raise KernelError(f"{what}: {name} must be a contiguous {dims}-dimensional tensor of {dtype} on the cache's device, is "
+                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _take_cache(what: str, cache_layer: torch.Tensor, num_kv_heads: int, head_dim: int, page_size: int, positions: torch.Tensor,
+                token_seq: torch.Tensor, block_table: torch.Tensor) -> int:
+    """Checks the cache and the rows' metadata; returns the device."""
+    if head_dim <= 0 or head_dim % 16 or head_dim > 256 or num_kv_heads <= 0 or page_size <= 0:
+        raise KernelError(f"{what}: {num_kv_heads} KV heads of {head_dim} in pages of {page_size} are not taken (head sizes are "
+                          f"multiples of 16 up to 256)")
+    if not cache_layer.is_cuda:
+        raise KernelError(f"{what}: the cache must be a CUDA tensor")
+    device = cache_layer.get_device()
+    if device != torch.cuda.current_device():
+        raise KernelError(f"{what}: the cache is on device {device}, the current device is {torch.cuda.current_device()}")
+    _take(what, cache_layer, "cache_layer", torch.uint8, 2, device)
+    if cache_layer.shape[1] != kv8_page_bytes(num_kv_heads, page_size, head_dim) or cache_layer.data_ptr() % 16:
+        raise KernelError(f"{what}: the cache must be 16-byte aligned pages of {kv8_page_bytes(num_kv_heads, page_size, head_dim)} "
+                          f"bytes, is {tuple(cache_layer.shape)}")
+    _take(what, positions, "positions", torch.int32, 1, device)
+    _take(what, token_seq, "token_seq", torch.int32, 1, device)
+    _take(what, block_table, "block_table", torch.int32, 2, device)
+    if positions.shape[0] < token_seq.shape[0] or block_table.numel() == 0:
+        raise KernelError(f"{what}: fewer positions than rows, or an empty block table")
+    return device
+
+
+def rope_kv8_store(qkv: torch.Tensor, q_out: torch.Tensor, cache_layer: torch.Tensor, positions: torch.Tensor,
+                   token_seq: torch.Tensor, block_table: torch.Tensor, cos_sin: Optional[torch.Tensor], pairing: int,
+                   num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> None:
+    """The rows of a stacked Q, K, V projection (``[T, (nh + 2 nkv) hd]`` in the type of ``q_out`` or 32-bit, or 32-bit partial sums
+    ``[S, T, ...]`` added in order): Q rotated into ``q_out [T, nh*hd]``, K rotated and V rounded to 8 bits into slot
+    ``positions[t] % page_size`` of page ``block_table[token_seq[t], positions[t] // page_size]``.  All in 32 bits, each result
+    rounded once.  ``cos_sin [T, hd/2, 2]`` (None: no rotation); ``pairing`` as for :func:`rope_kv_store` (0: element i with
+    i + hd/2; 1: neighbours; 2: neighbours in the input, halves in the result).  A row without a page (position or sequence outside
+    the block table, page id outside the cache) is not kept, its query is written all the same.  A number that is not finite is kept as
+    NaN.  Two rows of one step must not name the same slot."""
+    what = "rope_kv8_store"
+    device = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
+    T = token_seq.shape[0]
+    width = (num_heads + 2 * num_kv_heads) * head_dim
+    act, dt = _CODES.get(q_out.dtype), _CODES.get(qkv.dtype)
+    if act is None or dt is None or (dt == AP_BF16 and act == AP_F32) or num_heads <= 0:
+        raise KernelError(f"{what}: types {qkv.dtype} and {q_out.dtype} (float32 or bfloat16, the input no narrower than 32 bits "
+                          f"where the queries are)")
+    _take(what, qkv, "qkv", torch.float32 if qkv.dim() == 3 else qkv.dtype, qkv.dim(), device)
+    _take(what, q_out, "q_out", q_out.dtype, 2, device)
+    if qkv.dim() not in (2, 3) or qkv.shape[-2] != T or qkv.shape[-1] != width or qkv.shape[0] == 0 != T or q_out.shape[0] < T \
+            or q_out.shape[1] != num_heads * head_dim:
+        raise KernelError(f"{what}: shapes disagree: qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)}, {T} rows of {num_heads} + "
+                          f"2 x {num_kv_heads} heads of {head_dim}")
+    if qkv.data_ptr() % 16 or q_out.data_ptr() % 16:
+        raise KernelError(f"{what}: qkv and q_out must be 16-byte aligned")
+    cs = 0
+    if cos_sin is not None:
+        _take(what, cos_sin, "cos_sin", torch.float32, 3, device)
+        if cos_sin.shape[0] < T or cos_sin.shape[1] != head_dim // 2 or cos_sin.shape[2] != 2 or cos_sin.data_ptr() % 16:
+            raise KernelError(f"{what}: cos_sin must be 16-byte aligned [T, head_dim/2, 2], is {tuple(cos_sin.shape)}")
+        cs = cos_sin.data_ptr()
+    if pairing not in (0, 1, 2):
+        raise KernelError(f"{what}: unknown pairing {pairing}")
+    S = qkv.shape[0] if qkv.dim() == 3 else 1
+    call(core(), "ap_rope_kv8_store", qkv.data_ptr(), dt, S, T * width, q_out.data_ptr(), act, cache_layer.data_ptr(),
+         cache_layer.shape[0], cache_layer.shape[1], positions.data_ptr(), token_seq.data_ptr(), block_table.data_ptr(),
+         block_table.shape[1], block_table.shape[0], cs, int(pairing), T, num_heads, num_kv_heads, head_dim, page_size,
+         stream_handle())
+
+
+def kv8_read(cache_layer: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor, block_table: torch.Tensor,
+             k_out: Optional[torch.Tensor], v_out: Optional[torch.Tensor], num_kv_heads: int, head_dim: int,
+             page_size: int) -> None:
+    """The keys and values of cached rows: row ``r`` of ``k_out`` and ``v_out`` (float32 or bfloat16 ``[rows, nkv*hd]``, either may be
+    None) gets position ``positions[r]`` of sequence ``token_seq[r]``, exactly what the cache stands for (bfloat16 holds it too).
+    A row without a page reads as zeros."""
+    what = "kv8_read"
+    device = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
+    T = token_seq.shape[0]
+    some = k_out if k_out is not None else v_out
+    if some is None:
+        return
+    code = _CODES.get(some.dtype)
+    if code is None:
+        raise KernelError(f"{what}: outputs of {some.dtype} are not taken (float32, bfloat16)")
+    ptr = [0, 0]
+    for i, t in enumerate((k_out, v_out)):
+        if t is not None:
+            _take(what, t, "an output", some.dtype, 2, device)
+            if t.shape[0] < T or t.shape[1] != num_kv_heads * head_dim or t.data_ptr() % 16:
+                raise KernelError(f"{what}: outputs must be 16-byte aligned [rows, {num_kv_heads * head_dim}], one is {tuple(t.shape)}")
+            ptr[i] = t.data_ptr()
+    call(core(), "ap_kv8_read", cache_layer.data_ptr(), cache_layer.shape[0], cache_layer.shape[1], positions.data_ptr(),
+         token_seq.data_ptr(), block_table.data_ptr(), block_table.shape[1], block_table.shape[0], ptr[0], ptr[1], code, T,
+         num_kv_heads, head_dim, page_size, stream_handle())
+
+
+def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor, block_table: torch.Tensor,
+                  token_seq: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
+                  page_size: int, scale: float, window: int = 0, seq_start: Optional[torch.Tensor] = None,
+                  query_lens: Optional[Sequence[int]] = None, max_context: int = 0, scratch=None,
+                  mean_context: int = 0) -> None:
+    """Causal attention of every row of ``q [T, nh*hd]`` over its sequence's keys in the 8-bit cache; arguments as for
+    :func:`attention`, with ``page_size`` beside the flat pages.  Scores, softmax and sums are 32-bit.  A row sees the keys at and
+    before its position (the last ``window`` of them, 0: all) whose page is there; one that sees none gets zeros.  The rows of a
+    sequence follow one another and so do their positions."""
+    what = "attention_kv8"
+    device = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
+    T = token_seq.shape[0]
+    code = _CODES.get(q.dtype)
+    if code is None or num_heads <= 0 or num_heads % num_kv_heads or window < 0:
+        raise KernelError(f"{what}: {num_heads} heads on {num_kv_heads} KV heads in {q.dtype}, window {window}")
+    _take(what, q, "q", q.dtype, 2, device)
+    _take(what, out, "out", q.dtype, 2, device)
+    if q.shape[0] < T or q.shape[1] != num_heads * head_dim or out.shape != q.shape or q.data_ptr() % 16 or out.data_ptr() % 16:
+        raise KernelError(f"{what}: q {tuple(q.shape)} and out {tuple(out.shape)} must be 16-byte aligned rows of {num_heads} heads of "
+                          f"{head_dim}, {T} at least")
+    if seq_start is not None and query_lens is not None:
+        _take(what, seq_start, "seq_start", torch.int32, 1, device)
+        if seq_start.shape[0] != len(query_lens) + 1 or sum(query_lens) != T or block_table.shape[0] < len(query_lens):
+            raise KernelError(f"{what}: seq_start, query_lens and the block table do not describe the rows")
+    call(library.attention(head_dim), "ap_attention_kv8_rows", q.data_ptr(), out.data_ptr(), code, cache_layer.data_ptr(),
+         cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr(), block_table.shape[1], block_table.shape[0],
+         token_seq.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, head_dim, page_size, float(scale), int(window),
+         stream_handle())

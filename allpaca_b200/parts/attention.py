@@ -11,7 +11,8 @@ product here: their weights are stacked ``[Wq; Wk; Wv]`` at load.
 
 A ``window`` keeps only the last ``window`` keys visible, and lets the cache manager take
 back pages the window has passed.  ``shares_kv`` makes the layer read keys and values that
-another run of the order wrote: it then has no K/V weights.
+another run of the order wrote: it then has no K/V weights.  An engine may keep the keys and values in 8 bits
+(``BuildEnv.kv_dtype`` "fp8"): they are rounded as they are stored, and attention reads them as they are.
 """
 from __future__ import annotations
 
@@ -21,7 +22,7 @@ from typing import Dict, Mapping, Optional
 import torch
 
 from .. import ops
-from .base import BuildEnv, CacheNeed, KVNeed, LayerCache, Mixer, PartError, WeightSpec, build, register
+from .base import BuildEnv, CacheNeed, KV8Need, KVNeed, LayerCache, Mixer, PartError, WeightSpec, build, register
 from .linear import Linear
 
 
@@ -63,6 +64,7 @@ class GroupedQueryAttention(Mixer):
         self.qkv = Linear(env, self.q_size + 2 * self.kv_size, self.hidden)
         self.o = Linear(env, self.hidden, self.q_size)
         self._interleaved = False
+        self.kv8 = env.kv_dtype == "fp8"
 
     # ---- weights --------------------------------------------------------
     def weights(self) -> Dict[str, WeightSpec]:
@@ -107,6 +109,8 @@ class GroupedQueryAttention(Mixer):
 
     # ---- cache ----------------------------------------------------------
     def cache_need(self) -> Optional[CacheNeed]:
+        if self.kv8:
+            return KV8Need(window=self.window, num_kv_heads=self.nkv, head_dim=self.hd)
         return KVNeed(self.nkv, self.hd, self.window)
 
     def parts(self):
@@ -144,7 +148,7 @@ class GroupedQueryAttention(Mixer):
         q = ws.get("attn.q", (T, self.q_size), self.env.dtype)
         table = self.position.rotation_for(step) if self.position is not None else None
         writes = cache.writes and not self.shares_kv
-        if (self.FUSE_ROPE and T <= self.FUSE_ROPE_MAX_ROWS and not self.shares_kv and self.qkv.fusable()
+        if (self.FUSE_ROPE and T <= self.FUSE_ROPE_MAX_ROWS and not self.shares_kv and not self.kv8 and self.qkv.fusable()
                 and (self.position is None or table is not None) and (table is None or table[1] == 1 or self._interleaved)):
             # few rows: rotation and the store of keys and values in the projection's epilogue
             cos_sin, pairing = table if table is not None else (None, 1)
@@ -163,6 +167,10 @@ class GroupedQueryAttention(Mixer):
         cos_sin, pairing = table if table is not None else (None, 0)
         if self._interleaved:
             pairing = 2                  # pairs side by side in the projection's output, halves in the result
+        if self.kv8 and writes:
+            ops.rope_kv8_store(qkv, q, cache.pages, step.positions, step.token_seq, step.block_tables[cache.group], cos_sin,
+                               pairing, self.nh, self.nkv, self.hd, self.env.page_size)
+            return self._attention(q, T, step, cache, ws)
         ops.rope_kv_store(
             qkv, q, cache.pages if writes else None, step.positions, step.token_seq,
             step.block_tables[cache.group] if writes else None, cos_sin, pairing,
@@ -171,6 +179,12 @@ class GroupedQueryAttention(Mixer):
 
     def _attention(self, q, T, step, cache, ws):
         attn = ws.get("attn.out", (T, self.q_size), self.env.dtype)
+        if self.kv8:
+            ops.attention_kv8(q, attn, cache.pages, step.block_tables[cache.group], step.token_seq, step.positions, self.nh,
+                              self.nkv, self.hd, self.env.page_size, self.scale, self.window or 0, seq_start=step.seq_start,
+                              query_lens=step.host_query_lens, max_context=step.max_decode_context_len or step.max_context_len,
+                              scratch=ws.get, mean_context=step.mean_context_len)
+            return attn
         ops.attention(q, attn, cache.pages, step.block_tables[cache.group], step.token_seq,
                       step.positions, self.nh, self.nkv, self.hd, self.scale,
                       self.window or 0, seq_start=step.seq_start, query_lens=step.host_query_lens,

@@ -76,6 +76,7 @@ class BuildEnv:
     workspace: "Workspace"
     page_size: int = 16                # tokens per cache page
     max_seqs: int = 1                  # state slots available to mixers with fixed-size state
+    kv_dtype: str = "auto"             # how keys and values are kept: "auto" (as `dtype`) or "fp8" (8 bits, a scale to a row)
 
 
 class Workspace:
@@ -154,6 +155,23 @@ class CacheNeed:
         for d in (*self.outer, *self.inner):
             n *= int(d)
         return n * torch.empty((), dtype=self.dtype or engine_dtype).element_size()
+
+
+@dataclass(frozen=True)
+class KV8Need(CacheNeed):
+    """Keys and values in 8 bits with a scale to a row: flat pages of bytes (see ``ops/kv8.py``).  Its kernels read only rows that
+    were written, so fresh pages are not cleared."""
+
+    num_kv_heads: int = 0
+    head_dim: int = 0
+    dtype: Optional[torch.dtype] = torch.uint8
+
+    def page_shape(self, page_size: int) -> Tuple[int, ...]:
+        from ..ops import kv8_page_bytes
+        return (kv8_page_bytes(self.num_kv_heads, int(page_size), self.head_dim),)
+
+    def page_bytes(self, page_size: int, engine_dtype: torch.dtype) -> int:
+        return self.page_shape(page_size)[0]
 
 
 def KVNeed(num_kv_heads: int, head_dim: int, window: Optional[int] = None) -> CacheNeed:
