@@ -118,6 +118,36 @@ def kv8_read(cache_layer: torch.Tensor, positions: torch.Tensor, token_seq: torc
          num_kv_heads, head_dim, page_size, stream_handle())
 
 
+_takes_split = {}
+
+
+def _splits(head_dim: int) -> bool:
+    """Whether the kernel for few rows is built for this head size."""
+    got = _takes_split.get(head_dim)
+    if got is None:
+        got = _takes_split[head_dim] = bool(library.attention(head_dim).ap_attention_kv8_split_supports(head_dim))
+    return got
+
+
+def plan_slices(ctas: int, keys: int, mean_keys: int):
+    """(key slices, warps to a CTA) of the kernel for few rows: ``ctas`` tiles x KV heads, rows that see up to ``keys`` keys."""
+    for n in (1, 2, 4, 8, 16):
+        if ctas * n >= 148 or keys <= 256 * n:
+            break
+    return n, 8 if ctas * n <= 148 else 4
+
+
+def _split(q, out, cache_layer, block_table, seq_start, positions, first_seq, nseq, tiles, num_heads, num_kv_heads, head_dim, page_size,
+           scale, window, keys, mean_keys) -> None:
+    group = num_heads // num_kv_heads
+    keys = min(keys, window + 32) if window else keys
+    nsplit, warps = plan_slices(tiles * num_kv_heads * -(-group // 8), keys, mean_keys)
+    call(library.attention(head_dim), "ap_attention_kv8_split", q.data_ptr(), out.data_ptr(), cache_layer.data_ptr(),
+         cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr() + 4 * first_seq * block_table.shape[1], block_table.shape[1],
+         0 if seq_start is None else seq_start.data_ptr() + 4 * first_seq, positions.data_ptr(), nseq, tiles, num_heads, num_kv_heads,
+         head_dim, page_size, float(scale), int(window), nsplit, warps, stream_handle())
+
+
 def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor, block_table: torch.Tensor,
                   token_seq: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
                   page_size: int, scale: float, window: int = 0, seq_start: Optional[torch.Tensor] = None,
@@ -142,6 +172,20 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
         _take(what, seq_start, "seq_start", torch.int32, 1, device)
         if seq_start.shape[0] != len(query_lens) + 1 or sum(query_lens) != T or block_table.shape[0] < len(query_lens):
             raise KernelError(f"{what}: seq_start, query_lens and the block table do not describe the rows")
+        if code == AP_BF16 and T and _splits(head_dim) and 0 < cache_layer.numel() < 1 << 36:
+            # sequences that bring one row each, then portions (one-row sequences further back ride along with them)
+            nd, nseq = 0, len(query_lens)
+            while nd < nseq and query_lens[nd] == 1:
+                nd += 1
+            if nd:
+                _split(q, out, cache_layer, block_table, None, positions, 0, nd, nd, num_heads, num_kv_heads, head_dim, page_size,
+                       scale, window, max_context or block_table.shape[1] * page_size, mean_context)
+            if nd < nseq:
+                per = library.attention(head_dim).ap_attention_kv8_split_tokens(num_heads, num_kv_heads)
+                _split(q, out, cache_layer, block_table, seq_start, positions, nd, nseq - nd,
+                       sum(-(-n // per) for n in query_lens[nd:]), num_heads, num_kv_heads, head_dim, page_size, scale, window,
+                       block_table.shape[1] * page_size, 0)
+            return
     call(library.attention(head_dim), "ap_attention_kv8_rows", q.data_ptr(), out.data_ptr(), code, cache_layer.data_ptr(),
          cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr(), block_table.shape[1], block_table.shape[0],
          token_seq.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, head_dim, page_size, float(scale), int(window),
