@@ -7,6 +7,9 @@ which no number of the row exceeds 448.  Pages are flat: ``cache_layer`` is uint
 """
 from __future__ import annotations
 
+import functools
+import itertools
+import random
 from typing import Optional, Sequence
 
 import torch
@@ -118,34 +121,59 @@ def kv8_read(cache_layer: torch.Tensor, positions: torch.Tensor, token_seq: torc
          num_kv_heads, head_dim, page_size, stream_handle())
 
 
-_takes_split = {}
+_nonces = itertools.count(random.getrandbits(61))
 
 
-def _splits(head_dim: int) -> bool:
-    """Whether the kernel for few rows is built for this head size."""
-    got = _takes_split.get(head_dim)
-    if got is None:
-        got = _takes_split[head_dim] = bool(library.attention(head_dim).ap_attention_kv8_split_supports(head_dim))
-    return got
+@functools.lru_cache(maxsize=None)
+def _sms(device: int) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
 
 
-def plan_slices(ctas: int, keys: int, mean_keys: int):
-    """(key slices, warps to a CTA) of the kernel for few rows: ``ctas`` tiles x KV heads, rows that see up to ``keys`` keys."""
-    for n in (1, 2, 4, 8, 16):
-        if ctas * n >= 148 or keys <= 256 * n:
-            break
-    return n, 8 if ctas * n <= 148 else 4
+@functools.lru_cache(maxsize=4096)
+def plan_rows(pairs: int, longest: int, mean: int, sms: int):
+    """(CTAs, CTAs to a cluster) of the kernel for single rows: ``pairs`` of a row and a KV head, of up to ``longest`` tiles of 64 keys,
+    ``mean`` on average.  Clusters (0: none) give every pair CTAs of its own.
+
+    Measured (one B200, pages scattered, us; a tile takes a CTA some 0.38 once its loads run): shared work costs 11 beside its tiles where
+    pairs outnumber the CTAs (64 rows of 2048 keys on 8 KV heads: 54.6, in clusters of one 69.9), 16 where every pair is cut (8 rows of
+    4096: 27.5; clusters of two 20.7, of four 29.0).  A pair to a cluster costs 5.5, and 1.2 for putting parts together (1 row of 4096:
+    clusters of eight 10.3, shared 18.2; of 300: of one 6.2, shared 10.5), but a CTA to an SM it leaves SMs idle (1 row of
+    32768: shared 27.6, of eight 30.6), and the longest row sets its time."""
+    best = ((16.0 if pairs < sms else 11.0) + 0.39 * pairs * mean / sms, max(1, min(sms, pairs * mean // 2)), 0)
+    for cluster, most in ((1, sms), (2, 64), (4, 32), (8, 16)):
+        if pairs <= most and (cluster == 1 or longest >= cluster):
+            best = min(best, (5.5 + 0.38 * -(-longest // cluster) + (1.2 if cluster > 1 else 0.0), pairs * cluster, cluster))
+    return best[1:]
 
 
-def _split(q, out, cache_layer, block_table, seq_start, positions, first_seq, nseq, tiles, num_heads, num_kv_heads, head_dim, page_size,
-           scale, window, keys, mean_keys) -> None:
+@functools.lru_cache(maxsize=None)
+def _single_rows_taken(head_dim: int, page_size: int) -> bool:
+    return bool(library.attention(head_dim).ap_attention_kv8_decode_takes(page_size))
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(num_heads: int, num_kv_heads: int, head_dim: int, ctas: int) -> int:
+    return library.attention(head_dim).ap_attention_kv8_decode_scratch(num_heads, num_kv_heads, ctas)
+
+
+def _rows(q, out, cache_layer, block_table, token_seq, positions, first, rows, num_heads, num_kv_heads, head_dim, page_size, scale,
+          window, longest, mean, scratch, device) -> None:
+    """Rows ``first`` to ``first + rows`` one by one, up to ``longest`` keys to a row and some ``mean``."""
+    lib = library.attention(head_dim)
     group = num_heads // num_kv_heads
-    keys = min(keys, window + 32) if window else keys
-    nsplit, warps = plan_slices(tiles * num_kv_heads * -(-group // 8), keys, mean_keys)
-    call(library.attention(head_dim), "ap_attention_kv8_split", q.data_ptr(), out.data_ptr(), cache_layer.data_ptr(),
-         cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr() + 4 * first_seq * block_table.shape[1], block_table.shape[1],
-         0 if seq_start is None else seq_start.data_ptr() + 4 * first_seq, positions.data_ptr(), nseq, tiles, num_heads, num_kv_heads,
-         head_dim, page_size, float(scale), int(window), nsplit, warps, stream_handle())
+    if window:
+        longest, mean = min(longest, window + 64), min(mean, window + 64)
+    step = 512
+    for r in range(first, first + rows, step):
+        n = min(step, first + rows - r)
+        ctas, cluster = plan_rows(n * num_kv_heads * -(-group // 8), -(-longest // 64), -(-mean // 64), _sms(device))
+        need = 0 if cluster else _scratch_bytes(num_heads, num_kv_heads, head_dim, ctas)
+        buf = None if cluster else scratch("attn.kv8", (need // 4,), torch.float32) if scratch is not None else \
+            torch.empty(need // 4, dtype=torch.float32, device=q.device)
+        call(lib, "ap_attention_kv8_decode", q.data_ptr() + 2 * r * q.shape[1], out.data_ptr() + 2 * r * q.shape[1],
+             cache_layer.data_ptr(), cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr(), block_table.shape[1],
+             block_table.shape[0], token_seq.data_ptr() + 4 * r, positions.data_ptr() + 4 * r, n, num_heads, num_kv_heads, head_dim,
+             page_size, float(scale), int(window), ctas, cluster, buf.data_ptr() if buf is not None else 0, need, next(_nonces) % (1 << 62) + 1, stream_handle())
 
 
 def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor, block_table: torch.Tensor,
@@ -172,20 +200,11 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
         _take(what, seq_start, "seq_start", torch.int32, 1, device)
         if seq_start.shape[0] != len(query_lens) + 1 or sum(query_lens) != T or block_table.shape[0] < len(query_lens):
             raise KernelError(f"{what}: seq_start, query_lens and the block table do not describe the rows")
-        if code == AP_BF16 and T and _splits(head_dim) and 0 < cache_layer.numel() < 1 << 36:
-            # sequences that bring one row each, then portions (one-row sequences further back ride along with them)
-            nd, nseq = 0, len(query_lens)
-            while nd < nseq and query_lens[nd] == 1:
-                nd += 1
-            if nd:
-                _split(q, out, cache_layer, block_table, None, positions, 0, nd, nd, num_heads, num_kv_heads, head_dim, page_size,
-                       scale, window, max_context or block_table.shape[1] * page_size, mean_context)
-            if nd < nseq:
-                per = library.attention(head_dim).ap_attention_kv8_split_tokens(num_heads, num_kv_heads)
-                _split(q, out, cache_layer, block_table, seq_start, positions, nd, nseq - nd,
-                       sum(-(-n // per) for n in query_lens[nd:]), num_heads, num_kv_heads, head_dim, page_size, scale, window,
-                       block_table.shape[1] * page_size, 0)
-            return
+    if code == AP_BF16 and T and 0 < cache_layer.numel() < 1 << 36 and _single_rows_taken(head_dim, page_size):
+        longest = max_context or block_table.shape[1] * page_size
+        _rows(q, out, cache_layer, block_table, token_seq, positions, 0, T, num_heads, num_kv_heads, head_dim, page_size, scale, window,
+              longest, min(mean_context or longest, longest), scratch, device)
+        return
     call(library.attention(head_dim), "ap_attention_kv8_rows", q.data_ptr(), out.data_ptr(), code, cache_layer.data_ptr(),
          cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr(), block_table.shape[1], block_table.shape[0],
          token_seq.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, head_dim, page_size, float(scale), int(window),

@@ -234,19 +234,22 @@ def attention(head_dim: int) -> ctypes.CDLL:
                 for name, args in _OPTIONAL_ATTN_SIGNATURES.items():
                     if hasattr(lib, name):
                         getattr(lib, name).argtypes = args
-                        getattr(lib, name).restype = c_int
+                        getattr(lib, name).restype = c_longlong if name in _LONG_RESULTS else c_int
                 _attn[head_dim] = lib
     return lib
 
 
+_LONG_RESULTS = ("ap_attention_kv8_decode_scratch",)
+
 _OPTIONAL_ATTN_SIGNATURES: Dict[str, list] = {
     "ap_attention_tc": [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _L, _F, _I, _I, _I, _I, _P, _P, _P],
     "ap_attention_tc_tokens_per_tile": [_I, _I],
-    # int ap_attention_kv8_split(q, out, cache, num_pages, page_bytes, block_table, max_blocks, seq_start, positions, nseq, tiles, nh,
-    #                            nkv, hd, P, scale, window, nsplit, warps, stream)
-    "ap_attention_kv8_split": [_P, _P, _P, _L, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P],
-    "ap_attention_kv8_split_supports": [_I],
-    "ap_attention_kv8_split_tokens": [_I, _I],
+    # int ap_attention_kv8_decode(q, out, cache, num_pages, page_bytes, block_table, max_blocks, nseq, token_seq, positions, T, nh, nkv,
+    #                             hd, P, scale, window, ctas, cluster, scratch, scratch_bytes, nonce, stream)
+    "ap_attention_kv8_decode": [_P, _P, _P, _L, _L, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _L, _L, _P],
+    "ap_attention_kv8_decode_scratch": [_I, _I, _I],
+    "ap_attention_kv8_decode_takes": [_I],
+    "ap_attention_kv8_decode_status": [],
     "ap_attention_tcgen05": [_P, _P, _P, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _L, _F, _I, _I, _P],
     "ap_attention_tcgen05_supports": [_I, _I, _I, _I],
     "ap_attention_tcgen05_tokens_per_tile": [_I, _I],

@@ -265,13 +265,12 @@ def test_refusals(ops):
     bad(att, q.float(), torch.zeros_like(q), cache, table, one, one, nh, nkv, hd, P, 1.0)
 
 
-@pytest.mark.parametrize("slices", [1, 2, 4, 8, 16])
-@pytest.mark.parametrize("warps", [4, 8])
-@pytest.mark.parametrize("nh,nkv,hd,P", [(8, 2, 128, 16), (16, 1, 128, 64), (40, 2, 64, 16), (6, 2, 96, 5), (8, 8, 32, 16)])
-def test_any_number_of_key_slices(ops, slices, warps, nh, nkv, hd, P, monkeypatch):
-    """Slices that hold many batches of keys, one or none, of single rows and of portions."""
+@pytest.mark.parametrize("ctas,cluster", [(1, 0), (2, 0), (3, 0), (7, 0), (31, 0), (100, 0), (148, 0), (400, 0), (1, 1), (1, 2), (1, 4), (1, 8), (1, 16)])
+@pytest.mark.parametrize("nh,nkv,hd,P", [(8, 2, 128, 16), (16, 1, 128, 64), (40, 2, 64, 16), (6, 2, 96, 5), (8, 8, 32, 16), (4, 1, 256, 7)])
+def test_any_cut_of_the_work(ops, ctas, cluster, nh, nkv, hd, P, monkeypatch):
+    """Runs of tiles that end inside a pair, hold many pairs, or none; pairs cut into many parts; all on scratch full of junk."""
     from allpaca_b200.ops import kv8
-    monkeypatch.setattr(kv8, "plan_slices", lambda *a: (slices, warps))
+    monkeypatch.setattr(kv8, "plan_rows", lambda *a: (ctas, cluster))
     for seqs in (DECODE, [(3000, 1), (700, 9), (333, 5), (3, 3)]):
-        c = plain.case(seqs, nh, nkv, hd, P, torch.bfloat16, seed=slices + hd)
+        c = plain.case(seqs, nh, nkv, hd, P, torch.bfloat16, seed=ctas + hd)
         check(run(ops, c, 0.09), c, 0.09)
