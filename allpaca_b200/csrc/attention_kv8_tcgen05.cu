@@ -1,0 +1,687 @@
+// Causal grouped-query attention of portions over the 8-bit paged cache (kv8.cuh) on the 5th-generation tensor cores, for head sizes
+// 64 and 128 (-DAP_HEAD_DIM): sequences that bring several new rows each, from two on, packed one behind the other.
+//
+// The arithmetic is that of attention_tcgen05_wide.cu: a CTA owns up to 256 rows, two tiles "a" and "b" of (128 / group) tokens x the
+// `group` query heads of one KV head, and every tile of 128 keys serves both; S and O live in tensor memory, the two tiles take turns
+// on the tensor cores while the other's softmax warps work (one row to a thread, P in bfloat16 over the S it came from, O scaled
+// down only when a row's maximum has grown by more than 2^8 over its reference).
+//
+// What is different is where K and V come from.  A loading warp brings the 8-bit numbers and the scale bytes of a tile's keys, or
+// values, into one of two raw buffers (TMA, a box to a page; 16 KB, half of what bfloat16 pages would move), and four more warps
+// turn them into the bfloat16 tiles that the products read: c * 2^e, exact, as scales are powers of two.  So nothing else changes, and no
+// precision is lost against a bfloat16 cache that holds the same values.  Per 16 numbers that is one 16-byte load, 40 conversions and
+// multiplications, two 16-byte stores, in an order that meets no bank twice (two rows to eight lanes); against the products'
+// 2750 cycles and more to a key tile of both query tiles it takes some 1000 of the issue slots of each scheduler.  Keys outside the range
+// that the CTA's rows see, and keys without a page, become zeros: what lies in their place may be NaN.
+//
+// Few rows leave most SMs idle: then the keys are cut into slices, a cluster of 2, 4 or 8 CTAs works on one set of rows, and the slices'
+// sums are added up through distributed shared memory, every CTA taking its share of the rows.  One launch, no scratch.
+//
+// Every wait is bounded; when one runs out a status word is raised and the results are void.
+//
+// Reference counterpart: attention_qtile_kernel (cuda/src/kernels.cu:1801), causal rule :1583-1585.
+#include "kv8.cuh"
+#include "tcgen05.cuh"
+#include <cuda.h>
+#include <math.h>
+
+#ifndef AP_HEAD_DIM
+#error "compile with -DAP_HEAD_DIM=<head size>"
+#endif
+
+#if (AP_HEAD_DIM == 64 || AP_HEAD_DIM == 128)
+
+#define HD AP_HEAD_DIM
+#define NHALF (HD / 64)
+#define BQ 128
+#define BKV 128
+#define SUB_BYTES (128 * 128)              // a [128 rows x 64 bf16] sub-tile
+#define Q_BYTES (NHALF * SUB_BYTES)        // one query tile
+#define KV_BYTES (NHALF * SUB_BYTES)       // K (or V) of one tile
+#define RAW_BYTES (BKV * HD)               // the same in 8 bits
+#define T8_THREADS 512                     // 2 x 4 softmax warps; loading warp, MMA warp, two idle ones; four converting warps
+#define T8_LOAD_WARP 8
+#define T8_MMA_WARP 9
+#define T8_CONVERT_WARP 12
+#define T8_TMEM_COLS 512                   // S_a, S_b: 2 x 128 columns; O_a, O_b: 2 x HD
+#define T8_O_COL 256
+#define T8_PITCH (HD + 4)                  // a row of sums that slices exchange, in floats
+#define LOG2E_F 1.4426950408889634f
+#define T8_ERR_WAIT 9
+
+static __device__ int g_t8_status;
+
+__device__ __forceinline__ float t8_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x by the special-function unit; exactly 0 for x = -inf
+__device__ __forceinline__ float t8_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct AttnT8Params {
+    bf16* out;
+    const uint8_t* cache;
+    const int* block_table;
+    const int* seq_start;
+    const int* positions;
+    size_t page_bytes;
+    int num_pages, max_blocks, nseq, nh, nkv, P, window, group, tokens_per_tile;   // tokens_per_tile: of one query tile
+    int nsplit;
+    float scale_log2;
+};
+
+struct T8Smem {
+    static constexpr int kQ = 0;                                  // tile a, tile b
+    static constexpr int kK = kQ + 2 * Q_BYTES;
+    static constexpr int kV = kK + 2 * KV_BYTES;
+    static constexpr int kRaw = kV + 2 * KV_BYTES;                // two buffers
+    static constexpr int kScale = kRaw + 2 * RAW_BYTES;           // their scale bytes
+    static constexpr int kBars = kScale + 2 * BKV;
+    static constexpr int kTotal = kBars + 256 + 1024;             // + alignment slack
+    // slices: [row of both tiles][T8_PITCH], then [row][maximum, sum], over Q, K and V when all is done
+    static constexpr int kSums = 0;
+    static constexpr int kStats = 2 * BQ * T8_PITCH * 4;
+};
+static_assert(T8Smem::kStats + 2 * BQ * 8 <= T8Smem::kRaw, "the slices' sums lie over the tiles");
+static_assert(T8Smem::kTotal <= 227 * 1024, "shared memory");
+
+template <bool SPLIT>
+__global__ void __launch_bounds__(T8_THREADS, 1)
+attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv,
+                             const AttnT8Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = (uint64_t*)(smem + T8Smem::kBars);
+    uint64_t* q_full = bars + 0;
+    uint64_t* raw_full = bars + 1;                        // [buffer]
+    uint64_t* raw_free = raw_full + 2;                    // [buffer]
+    uint64_t* k_full = raw_free + 2;                      // [stage]
+    uint64_t* v_full = k_full + 2;                        // [stage]
+    uint64_t* kv_free = v_full + 2;                       // [key tile & 1]: V of that tile and K of the next are read
+    uint64_t* s_full = kv_free + 2;                       // [query tile]
+    uint64_t* p_ready = s_full + 2;                       // [query tile]
+    uint64_t* o_full = p_ready + 2;                       // [query tile]: the last product into O is done
+    uint32_t* tmem_slot = (uint32_t*)(o_full + 2);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    volatile int* s_seq = (volatile int*)(tmem_slot + 2);
+    volatile int* s_tile = (volatile int*)(tmem_slot + 3);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per_cta = 2 * p.tokens_per_tile;            // tokens of one CTA
+
+    if (threadIdx.x == 0) {
+        // late portions of a sequence have the most keys to walk: hand them out first
+        // (the KV head is the fast index of the grid: all heads of the longest portions start first)
+        int t = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)p.nkv), found = -1;
+        for (int s = 0; s < p.nseq; ++s) {
+            const int n = p.seq_start[s + 1] - p.seq_start[s];
+            const int nt = (n + per_cta - 1) / per_cta;
+            if (t < nt) { found = s; break; }
+            t -= nt;
+        }
+        *s_seq = *(volatile int*)&g_t8_status != 0 ? -1 : found;       // (after an earlier failure: nothing, but the barriers)
+        *s_tile = t;
+        tc::mbar_init(q_full, 1);
+        for (int x = 0; x < 2; ++x) {
+            tc::mbar_init(&raw_full[x], 1 + 32);          // what TMA brings, and the lanes' scale bytes
+            tc::mbar_init(&raw_free[x], 4);
+            tc::mbar_init(&k_full[x], 4);
+            tc::mbar_init(&v_full[x], 4);
+            tc::mbar_init(&kv_free[x], 1);
+            tc::mbar_init(&s_full[x], 1);
+            tc::mbar_init(&p_ready[x], 4);                // one arrival per warp of the tile's group
+            tc::mbar_init(&o_full[x], 1);
+        }
+        *abort_flag = 0;
+        tc::fence_barrier_init();
+        tc::prefetch_tensormap(&tmap_q);
+        tc::prefetch_tensormap(&tmap_kv);
+    }
+    // the second query tile starts as zeros: it may not exist
+    for (int i = threadIdx.x; i < Q_BYTES / 16; i += T8_THREADS)
+        reinterpret_cast<uint4*>(smem + T8Smem::kQ + Q_BYTES)[i] = make_uint4(0, 0, 0, 0);
+    tc::fence_proxy_async();
+    if (warp == T8_MMA_WARP) tc::tmem_alloc(tmem_slot, T8_TMEM_COLS);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const int seq = *s_seq;
+    const uint32_t tmem_base = *tmem_slot;
+    const bool active = seq >= 0;
+
+    // geometry of this CTA (identical in every thread)
+    const int G = p.group;
+    int row0 = 0, ntok = 0, kmax = -1, kmin = 0, kvh = 0, head0 = 0;
+    if (active) {
+        row0 = p.seq_start[seq] + *s_tile * per_cta;
+        ntok = min(per_cta, p.seq_start[seq + 1] - row0);
+        kvh = (int)(blockIdx.x % (unsigned)p.nkv);
+        head0 = kvh * G;
+    }
+    const bool has_b = ntok > p.tokens_per_tile;          // the second query tile holds rows
+    ap_pdl_wait();
+    if (active) {
+        kmax = min(p.positions[row0 + ntok - 1], p.max_blocks * p.P - 1);
+        const int first = p.positions[row0];
+        kmin = (p.window > 0 && first - p.window + 1 > 0) ? first - p.window + 1 : 0;
+    }
+    int t_lo = kmin / BKV, t_hi = active ? kmax / BKV : -1;
+    if (SPLIT) {
+        const int each = (t_hi - t_lo + 1 + p.nsplit - 1) / p.nsplit;
+        t_lo += (int)blockIdx.y * each;
+        t_hi = min(t_hi, t_lo + each - 1);
+    }
+    const int ntiles = max(t_hi - t_lo + 1, 0);
+    const int* table = p.block_table + (size_t)(active ? seq : 0) * p.max_blocks;
+    const int n_pages = p.P < BKV ? BKV / p.P : 1, page_rows = BKV / n_pages;      // of a tile
+    // the page of lane `lane` of tile `it` (-1: none)
+    auto page_of = [&](int it) {
+        const int key0 = (t_lo + it) * BKV + lane * page_rows;
+        if (it >= ntiles || lane >= n_pages || key0 > kmax || key0 + page_rows - 1 < kmin) return -1;
+        const int page = table[key0 / p.P];
+        return page < p.num_pages ? page : -1;
+    };
+    // Tiles go K 0, K 1, V 0, K 2, V 1, ...: K runs one tile ahead of V.  The n-th of them:
+    auto nth = [&](int n, int& it, int& which) {
+        if (n == 0) { it = 0; which = 0; return; }
+        if (ntiles == 1) { it = 0; which = 1; return; }
+        if (n == 2 * ntiles - 1) { it = ntiles - 1; which = 1; return; }
+        it = (n & 1) ? (n + 1) / 2 : n / 2 - 1;
+        which = (n & 1) ? 0 : 1;
+    };
+
+    // Registers move from the warps that issue and convert to the softmax warps, which hold a row of 128 scores each (the unit of such a
+    // move is four warps): 2 x 192 + 64 + 64 = 512 to a thread of each, what the launch holds.
+    if (warp >= 8 && warp < T8_CONVERT_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == T8_LOAD_WARP) {
+        if (active && ntiles > 0) {
+            if (lane == 0) {
+                tc::mbar_expect_tx(q_full, (uint32_t)((has_b ? 2 : 1) * Q_BYTES));
+                for (int x = 0; x < (has_b ? 2 : 1); ++x)
+                    for (int h = 0; h < NHALF; ++h)
+                        tc::tma_load_3d(smem + T8Smem::kQ + x * Q_BYTES + h * SUB_BYTES, &tmap_q, h * 64, head0,
+                                        row0 + x * p.tokens_per_tile, q_full);
+            }
+            const int s_page = lane * 4 / page_rows;       // the page of this lane's four scale bytes
+            const uint8_t* const scales = p.cache + (size_t)2 * p.nkv * p.P * HD + (lane * 4 & (page_rows - 1));
+            int n = 0;
+            auto load = [&](int it, int which, int page) -> bool {
+                const int b = n & 1;
+                const int there = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                const int page_s = __shfl_sync(0xffffffffu, page, s_page);
+                int fine = 1;
+                if (lane == 0) {
+                    if (*abort_flag) fine = 0;
+                    if (fine && !tc::mbar_wait(&raw_free[b], (uint32_t)((n >> 1) & 1) ^ 1)) {
+                        *abort_flag = 1;
+                        atomicExch(&g_t8_status, T8_ERR_WAIT);
+                        fine = 0;
+                    }
+                    if (fine) tc::mbar_expect_tx(&raw_full[b], (uint32_t)(there * page_rows * HD));
+                }
+                fine = __shfl_sync(0xffffffffu, fine, 0);
+                if (!fine) return false;
+                const int krow = (which * p.nkv + kvh) * p.P + (p.P > BKV ? (t_lo + it) * BKV % p.P : 0);
+                if (page >= 0)
+                    tc::tma_load_3d(smem + T8Smem::kRaw + b * RAW_BYTES + lane * page_rows * HD, &tmap_kv, 0, krow, page, &raw_full[b]);
+                const uint8_t* sc = scales + (size_t)max(page_s, 0) * p.page_bytes + krow;
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(tc::smem_addr(smem + T8Smem::kScale + b * BKV + lane * 4)),
+                             "l"(sc), "r"(page_s >= 0 ? 4 : 0) : "memory");
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(tc::smem_addr(&raw_full[b])) : "memory");
+                ++n;
+                return true;
+            };
+            // K runs one tile ahead of V; the block table is read four tiles ahead of its use
+            int page_v = page_of(0);
+            int q0 = page_of(1), q1 = page_of(2), q2 = page_of(3), q3 = page_of(4);
+            bool fine = load(0, 0, page_v);
+            for (int it = 0; it < ntiles && fine; ++it) {
+                const int page_k = q0;
+                q0 = q1; q1 = q2; q2 = q3;
+                q3 = page_of(it + 5);
+                if (it + 1 < ntiles) fine = load(it + 1, 0, page_k);
+                if (fine) fine = load(it, 1, page_v);
+                page_v = page_k;
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+    } else if (warp == T8_MMA_WARP) {
+        if (lane == 0 && active && ntiles > 0) {
+            constexpr uint32_t idesc_s = tc::instr_desc_bf16_f32(BQ, BKV);
+            constexpr uint32_t idesc_o = tc::instr_desc_bf16_f32_b_mn(BQ, HD);
+            const int nx = has_b ? 2 : 1;
+            // S_x = Q_x K^T of key tile `it`
+            auto scores = [&](int it, int x) {
+                const int s = it & 1;
+#pragma unroll
+                for (int h = 0; h < NHALF; ++h) {
+                    const uint64_t qd = tc::smem_desc_k_major_sw128(smem + T8Smem::kQ + x * Q_BYTES + h * SUB_BYTES);
+                    const uint64_t kd = tc::smem_desc_k_major_sw128(smem + T8Smem::kK + s * KV_BYTES + h * SUB_BYTES);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tc::mma_bf16(tmem_base + (uint32_t)(x * BKV), qd + 2 * k, kd + 2 * k, idesc_s, (h > 0 || k > 0) ? 1u : 0u);
+                }
+                tc::mma_commit(&s_full[x]);
+            };
+            bool ok = tc::mbar_wait(q_full, 0);
+            if (ok) ok = tc::mbar_wait(&k_full[0], 0);
+            if (ok) {
+                tc::fence_after_sync();
+                for (int x = 0; x < nx; ++x) scores(0, x);
+                tc::mma_commit(&kv_free[1]);              // "tile -1": K of tile 0 is read
+            }
+            for (int it = 0; it < ntiles && ok; ++it) {
+                const int sv = it & 1;
+                const bool more = it + 1 < ntiles;
+                ok = tc::mbar_wait(&v_full[sv], (uint32_t)((it >> 1) & 1)) &&
+                     (!more || tc::mbar_wait(&k_full[(it + 1) & 1], (uint32_t)(((it + 1) >> 1) & 1)));
+                if (!ok || *abort_flag) break;
+                const uint64_t vd = tc::smem_desc_mn_major_sw128(smem + T8Smem::kV + sv * KV_BYTES, SUB_BYTES);
+                for (int x = 0; x < nx && ok; ++x) {
+                    // O_x += P_x V as soon as the tile's group has written P_x (and scaled O_x down where a row's reference
+                    // maximum moved); then S_x of the next key tile, which the group turns to while the other tile's products run
+                    ok = tc::mbar_wait(&p_ready[x], (uint32_t)(it & 1));
+                    if (!ok) break;
+                    tc::fence_after_sync();
+                    const uint32_t pt = tmem_base + (uint32_t)(x * BKV);      // P_x lies over S_x
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)
+                        tc::mma_bf16_a_tmem(tmem_base + (uint32_t)(T8_O_COL + x * HD), pt + (uint32_t)(ks * 8),
+                                            vd + (uint64_t)(ks * (16 * 128 / 16)), idesc_o, (it > 0 || ks > 0) ? 1u : 0u);
+                    if (!more) tc::mma_commit(&o_full[x]);
+                    if (more) scores(it + 1, x);
+                }
+                if (!ok) break;
+                tc::mma_commit(&kv_free[it & 1]);
+            }
+            if (!ok && !*abort_flag) {
+                *abort_flag = 1;
+                atomicExch(&g_t8_status, T8_ERR_WAIT);
+            }
+        }
+    }
+    } else if (warp >= T8_CONVERT_WARP) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (active && ntiles > 0) {
+        // Lane l of sixteen takes 16-byte chunk l & 7 (head size 64: l & 3) of one of two rows: eight lanes read 128 bytes in a row, and what
+        // they write, even chunks of the one row and odd ones of the other, lies in different banks.
+        const int cw = warp - T8_CONVERT_WARP;
+        const int q = HD == 128 ? lane & 7 : lane & 3;
+        const int r2 = HD == 128 ? (lane >> 4) * 2 + (((lane >> 2) ^ (lane >> 3)) & 1) : lane >> 2;     // of the 4 (8) rows of a warp's run
+        constexpr int kRows = HD == 128 ? 4 : 8;
+        bool ok = true;
+        for (int n = 0; n < 2 * ntiles && ok; ++n) {
+            int it, which;
+            nth(n, it, which);
+            const int b = n & 1, s = it & 1;
+            ok = __all_sync(0xffffffffu, tc::mbar_wait(&raw_full[b], (uint32_t)((n >> 1) & 1)));
+            // the stage's last readers: K of tile j - 2 in turn j - 3, V of tile j - 2 in turn j - 2 (kv_free is given one arrival
+            // before the first turn, "tile -1", and one at the end of every turn)
+            const int after = which ? it - 2 : it - 3;
+            if (ok && it >= 2) ok = __all_sync(0xffffffffu, tc::mbar_wait(&kv_free[after & 1], (uint32_t)(((after + (after & 1)) >> 1) & 1)));
+            if (!ok) {
+                if (!*abort_flag) {
+                    *abort_flag = 1;
+                    atomicExch(&g_t8_status, T8_ERR_WAIT);
+                }
+                break;
+            }
+            const uint8_t* raw = smem + T8Smem::kRaw + b * RAW_BYTES;
+            const uint8_t* scale = smem + T8Smem::kScale + b * BKV;
+            uint8_t* to = smem + (which ? T8Smem::kV : T8Smem::kK) + s * KV_BYTES + (q >> 2) * SUB_BYTES;
+            const int key0 = (t_lo + it) * BKV;
+#pragma unroll 4
+            for (int i = 0; i < BKV / (4 * kRows); ++i) {
+                const int r = (i * 4 + cw) * kRows + r2;
+                const uint4 u = *reinterpret_cast<const uint4*>(raw + r * HD + q * 16);
+                const uint32_t byte = scale[r];
+                const bool is = byte != 0 && key0 + r >= kmin && key0 + r <= kmax;
+                const float2 f2 = make_float2(kv8_scale(byte), kv8_scale(byte));
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                uint32_t o[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float4 f = kv8_unpack(w[k]);
+                    const float2 lo = __fmul2_rn(make_float2(f.x, f.y), f2), hi = __fmul2_rn(make_float2(f.z, f.w), f2);
+                    __nv_bfloat162 a = __floats2bfloat162_rn(lo.x, lo.y), c = __floats2bfloat162_rn(hi.x, hi.y);
+                    o[2 * k] = is ? *reinterpret_cast<uint32_t*>(&a) : 0u;
+                    o[2 * k + 1] = is ? *reinterpret_cast<uint32_t*>(&c) : 0u;
+                }
+                const int c0 = (q & 3) * 2;
+                *reinterpret_cast<uint4*>(to + r * 128 + ((c0 ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(to + r * 128 + (((c0 + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            tc::fence_proxy_async();                       // the products read through the other proxy
+            __syncwarp();
+            if (lane == 0) {
+                tc::mbar_arrive(&raw_free[b]);
+                tc::mbar_arrive(which ? &v_full[s] : &k_full[s]);
+            }
+        }
+    }
+    } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    if (active && (warp < 4 || has_b)) {
+        // ---- softmax: warps 0..3 own query tile a, warps 4..7 tile b; one row per thread ----
+        const int x = warp >> 2;
+        const int qtr = warp & 3;
+        const int r = qtr * 32 + lane;                 // row of the tile = (token r / G, head r % G)
+        const int tok = x * p.tokens_per_tile + r / G, hq = r % G;
+        const bool rvalid = tok < ntok;
+        const uint32_t lane_base = tmem_base + ((uint32_t)(qtr * 32) << 16);
+        const uint32_t s_cols = lane_base + (uint32_t)(x * BKV);
+        const uint32_t o_cols = lane_base + (uint32_t)(T8_O_COL + x * HD);
+        const int qpos = p.positions[row0 + (rvalid ? tok : 0)];
+        float mref = -INFINITY, l = 0.f;               // the row's reference maximum (log2 units) and sum
+        bool ok = true;                                // the same in all lanes of a warp
+        int page = page_of(0);
+        for (int it = 0; it < ntiles; ++it) {
+            const int k0 = (t_lo + it) * BKV;
+            // pages that the rows' keys lie in and that are not there (rare: a caller gives them back behind a window only)
+            const int mine = k0 + lane * page_rows;
+            const uint32_t gone = __ballot_sync(0xffffffffu, lane < n_pages && page < 0 && mine <= kmax && mine + page_rows - 1 >= kmin);
+            page = page_of(it + 1);
+            // tcgen05.ld and .st are warp-wide instructions: whatever decides whether one runs is a vote
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_full[x], (uint32_t)(it & 1)))) { ok = false; break; }
+            tc::fence_after_sync();
+            const bool row_all = rvalid && k0 + BKV - 1 <= qpos && (p.window <= 0 || qpos - k0 < p.window);
+            const bool row_none = !rvalid || k0 > qpos || (p.window > 0 && qpos - (k0 + BKV - 1) >= p.window);
+            const bool all_visible = __all_sync(0xffffffffu, row_all) && gone == 0;
+            const bool none_visible = __all_sync(0xffffffffu, row_none);
+            float lsum = 0.f;
+            if (none_visible) {
+                // nothing of this tile is for this warp's rows: P = 0
+                uint32_t zero[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) zero[j] = 0u;
+                tc::tmem_st_x32(s_cols, zero);
+                tc::tmem_st_x32(s_cols + 32u, zero);
+            } else {
+                // the row's 128 scores, masked ones as -inf (their probability below is exactly zero)
+                uint32_t v[128];
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) tc::tmem_ld_x32(s_cols + (uint32_t)c, v + c);
+                tc::tmem_ld_wait();
+                if (!all_visible) {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j) {
+                        const int kpos = k0 + j;
+                        const bool vis = rvalid && kpos <= qpos && (p.window <= 0 || qpos - kpos < p.window);
+                        v[j] = vis ? v[j] : 0xff800000u;
+                    }
+                    if (gone != 0) {
+#pragma unroll
+                        for (int j = 0; j < 128; j += 8) {                 // (pages are of eight rows at least)
+                            if (gone >> (j / page_rows) & 1u) {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) v[j + e] = 0xff800000u;
+                            }
+                        }
+                    }
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 128; j += 2)
+                    mx4[(j >> 1) & 3] = t8_max3(mx4[(j >> 1) & 3], __uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+                // the scale is positive: the maximum of the scaled scores is the scaled maximum
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+                const bool grow = mx > mref + 8.0f;            // also the row's first visible key
+                float alpha = 1.f;
+                if (grow) {
+                    alpha = t8_exp2(mref - mx);                // 0 when the row had no key yet
+                    mref = mx;
+                    l *= alpha;
+                }
+                if (it > 0 && __any_sync(0xffffffffu, grow)) {
+                    // scale this warp's rows of O_x down.  The product of the tile before into O_x is in: it was issued before the
+                    // scores whose arrival (s_full) this warp has seen, and an arrival stands for everything issued before it
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t w[32];
+                        tc::tmem_ld_x32(o_cols + (uint32_t)c, w);
+                        tc::tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
+                        tc::tmem_st_x32(o_cols + (uint32_t)c, w);
+                    }
+                    tc::tmem_st_wait();
+                }
+                // probabilities, two bfloat16 to a column, over the first half of S
+                const float muse = mref == -INFINITY ? 0.f : mref;
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(-muse, -muse);
+                float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int j = 0; j < 128; j += 2) {
+                    const float2 a = __ffma2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scale2, shift2);
+                    const float2 e = make_float2(t8_exp2(a.x), t8_exp2(a.y));
+                    l2[(j >> 1) & 1] = __fadd2_rn(l2[(j >> 1) & 1], e);
+                    __nv_bfloat162 b2 = __floats2bfloat162_rn(e.x, e.y);
+                    v[j >> 1] = *reinterpret_cast<uint32_t*>(&b2);
+                }
+                lsum = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+                tc::tmem_st_x32(s_cols, v);
+                tc::tmem_st_x32(s_cols + 32u, v + 32);
+            }
+            l += lsum;
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            __syncwarp();                       // every lane's part of P is written: one arrival for the warp
+            if (lane == 0) tc::mbar_arrive(&p_ready[x]);
+        }
+        // the last product into O_x, then the row goes out, or to the other slices
+        if (ok && ntiles > 0 && !__all_sync(0xffffffffu, tc::mbar_wait(&o_full[x], 0))) ok = false;
+        tc::fence_after_sync();
+        if (!ok) {
+            if (!*abort_flag) {
+                *abort_flag = 1;
+                atomicExch(&g_t8_status, T8_ERR_WAIT);
+            }
+        } else if (SPLIT) {
+            // (both query tiles' products are done when this one's are only where there is no other: wait for it before its operands are
+            // written over)
+            if (has_b && ntiles > 0 && !__all_sync(0xffffffffu, tc::mbar_wait(&o_full[x ^ 1], 0))) ok = false;
+            float* sums = reinterpret_cast<float*>(smem + T8Smem::kSums) + (size_t)(x * BQ + r) * T8_PITCH;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t w[32];
+                if (ntiles > 0) {
+                    tc::tmem_ld_x32(o_cols + (uint32_t)c, w);
+                    tc::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int d = 0; d < 32; ++d) w[d] = 0u;
+                }
+#pragma unroll
+                for (int d = 0; d < 32; d += 4)
+                    *reinterpret_cast<uint4*>(sums + c + d) = make_uint4(w[d], w[d + 1], w[d + 2], w[d + 3]);
+            }
+            *reinterpret_cast<float2*>(smem + T8Smem::kStats + (x * BQ + r) * 8) = make_float2(mref, l);
+        } else {
+            const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;     // (a sum that is not a number stays one)
+            bf16* dst = p.out + ((size_t)(row0 + (rvalid ? tok : 0)) * p.nh + head0 + hq) * HD;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t w[32];
+                if (ntiles > 0) {
+                    tc::tmem_ld_x32(o_cols + (uint32_t)c, w);
+                    tc::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int d = 0; d < 32; ++d) w[d] = 0u;
+                }
+                if (rvalid) {
+#pragma unroll
+                    for (int d = 0; d < 32; d += 8) {
+                        uint4 o8;
+                        __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o8);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o2[e] = __floats2bfloat162_rn(__uint_as_float(w[d + 2 * e]) * inv, __uint_as_float(w[d + 2 * e + 1]) * inv);
+                        *reinterpret_cast<uint4*>(dst + c + d) = o8;
+                    }
+                }
+            }
+        }
+    }
+    }
+    if (SPLIT) {
+        // Rows' sums of all slices, added up in the slices' order: row i of the CTAs' rows by CTA i % nsplit, a warp to a row
+        tc::cluster_sync();
+        const int rows = ntok * G, ns = p.nsplit;
+        for (int i = (int)blockIdx.y + ns * warp; i < rows; i += ns * (T8_THREADS / 32)) {
+            const int tok = i / G, hq = i - tok * G;
+            const uint32_t stats = tc::smem_addr(smem + T8Smem::kStats + i * 8);       // (tile b's rows lie behind tile a's)
+            const uint32_t sums = tc::smem_addr(smem + T8Smem::kSums) + (uint32_t)(i * T8_PITCH + lane * (HD / 32)) * 4u;
+            float M = -INFINITY, L = 0.f, O[HD / 32];
+#pragma unroll
+            for (int e = 0; e < HD / 32; ++e) O[e] = 0.f;
+            for (int z = 0; z < ns; ++z) {
+                const uint32_t st = tc::map_to_rank(stats, (uint32_t)z), su = tc::map_to_rank(sums, (uint32_t)z);
+                float m, l, o[HD / 32];
+                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m), "=f"(l) : "r"(st));
+                if constexpr (HD == 128)
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o[0]), "=f"(o[1]), "=f"(o[2]), "=f"(o[3]) : "r"(su));
+                else
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o[0]), "=f"(o[1]) : "r"(su));
+                const float m_new = fmaxf(M, m), use = m_new == -INFINITY ? 0.f : m_new;
+                const float f = t8_exp2(M - use), fz = t8_exp2(m - use);
+                M = m_new;
+                L = L * f + l * fz;
+#pragma unroll
+                for (int e = 0; e < HD / 32; ++e) O[e] = O[e] * f + o[e] * fz;
+            }
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            bf16* dst = p.out + ((size_t)(row0 + tok) * p.nh + head0 + hq) * HD + lane * (HD / 32);
+#pragma unroll
+            for (int e = 0; e < HD / 32; e += 2)
+                *reinterpret_cast<__nv_bfloat162*>(dst + e) = __floats2bfloat162_rn(O[e] * inv, O[e + 1] * inv);
+        }
+        tc::cluster_sync();                                // nobody leaves while its sums may be read
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    ap_pdl_trigger();
+    if (warp == T8_MMA_WARP) {
+        __syncwarp();
+        tc::tmem_dealloc(tmem_base, T8_TMEM_COLS);
+    }
+}
+
+// ---------------------------------------------------------------------------
+typedef CUresult (*T8EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                               CUtensorMapFloatOOBfill);
+
+static T8EncodeFn t8_encode_fn() {
+    static T8EncodeFn fn = nullptr;
+    if (!fn) {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = (T8EncodeFn)ptr;
+    }
+    return fn;
+}
+
+// 1 when ap_attention_kv8_tcgen05 takes this shape, else 0
+AP_EXPORT int ap_attention_kv8_tcgen05_takes(int nh, int nkv, int hd, int P) {
+    if (hd != HD || nkv <= 0 || nh % nkv) return 0;
+    const int g = nh / nkv;
+    if (g > 128 || 128 % g) return 0;
+    if (P < 8 || (P < BKV ? BKV % P : (P % BKV || P > 65536))) return 0;
+    return t8_encode_fn() != nullptr;
+}
+
+// tokens of one sequence that one CTA takes (two query tiles)
+AP_EXPORT int ap_attention_kv8_tcgen05_tokens(int nh, int nkv) { return 2 * (128 / (nh / nkv)); }
+
+// q: [T][nh][HD]; total_ctas: the sum over the sequences of ceil(rows / tokens of a CTA); nsplit: 1, 2, 4 or 8 key slices; scale > 0.
+AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cache, long long num_pages, long long page_bytes,
+                                       const int* block_table, int max_blocks, const int* seq_start, const int* positions, int nseq, int T,
+                                       int nh, int nkv, int hd, int P, float scale, int window, int total_ctas, int nsplit,
+                                       cudaStream_t stream) {
+    AP_REQUIRE(ap_attention_kv8_tcgen05_takes(nh, nkv, hd, P), "attention_kv8 (tcgen05): shape not supported: heads=%d kv_heads=%d "
+               "head_dim=%d page=%d", nh, nkv, hd, P);
+    AP_REQUIRE(T > 0 && nseq > 0 && total_ctas > 0 && max_blocks > 0, "attention_kv8 (tcgen05): bad sizes");
+    AP_REQUIRE(num_pages > 0 && num_pages < (1LL << 31) && page_bytes == kv8_page_bytes(nkv, P, HD), "attention_kv8: the pages do not match the heads");
+    AP_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)cache & 15) == 0 && ((uintptr_t)out & 15) == 0,
+               "attention_kv8 (tcgen05): operands must be 16-byte aligned");
+    AP_REQUIRE((long long)max_blocks * P < (1LL << 31) - 256, "attention_kv8: the block table names more than 2^31 keys");
+    AP_REQUIRE(scale > 0.f, "attention_kv8 (tcgen05): the scale must be positive");
+    AP_REQUIRE(nsplit == 1 || nsplit == 2 || nsplit == 4 || nsplit == 8, "attention_kv8: bad number of key slices %d", nsplit);
+    const int G = nh / nkv;
+    CUtensorMap mq, mkv;
+    {
+        cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)nh, (cuuint64_t)T};
+        cuuint64_t strides[2] = {(cuuint64_t)HD * 2, (cuuint64_t)nh * HD * 2};
+        cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(128 / G)};
+        cuuint32_t es[3] = {1, 1, 1};
+        AP_REQUIRE(t8_encode_fn()(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, es,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS,
+                   "attention_kv8 (tcgen05): cannot encode the query tensor map");
+    }
+    {
+        // [page][keys and values: head and row][number]; a box is one page's rows of one head
+        cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)2 * nkv * P, (cuuint64_t)num_pages};
+        cuuint64_t strides[2] = {(cuuint64_t)HD, (cuuint64_t)page_bytes};
+        cuuint32_t box[3] = {HD, (cuuint32_t)(P < BKV ? P : BKV), 1};
+        cuuint32_t es[3] = {1, 1, 1};
+        AP_REQUIRE(t8_encode_fn()(&mkv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(cache), dims, strides, box, es,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS,
+                   "attention_kv8 (tcgen05): cannot encode the cache tensor map");
+    }
+    static bool configured[64];
+    int dev = 0;
+    AP_REQUIRE(cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64, "attention_kv8: cannot tell the current device");
+    if (!configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(attention_kv8_tcgen05_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, T8Smem::kTotal);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(attention_kv8_tcgen05_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, T8Smem::kTotal);
+        AP_REQUIRE(e == cudaSuccess, "attention_kv8 (tcgen05): cannot reserve %d bytes of shared memory: %s", T8Smem::kTotal,
+                   cudaGetErrorString(e));
+        configured[dev] = true;
+    }
+    AttnT8Params p;
+    p.out = (bf16*)out; p.cache = (const uint8_t*)cache; p.block_table = block_table; p.seq_start = seq_start; p.positions = positions;
+    p.page_bytes = (size_t)page_bytes; p.num_pages = (int)num_pages; p.max_blocks = max_blocks; p.nseq = nseq; p.nh = nh; p.nkv = nkv;
+    p.P = P; p.window = window; p.group = G; p.tokens_per_tile = 128 / G; p.nsplit = nsplit;
+    p.scale_log2 = scale * LOG2E_F;
+    AP_REQUIRE((long long)total_ctas * nkv < (1LL << 31), "attention_kv8 (tcgen05): too many CTAs for the grid");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(total_ctas * nkv), nsplit);
+    cfg.blockDim = dim3(T8_THREADS);
+    cfg.dynamicSmemBytes = T8Smem::kTotal;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = ap_pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = nsplit;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = nsplit > 1 ? 2 : 1;
+    AP_CHECK_PDL_LAUNCH("attention_kv8_tcgen05", nsplit > 1 ? cudaLaunchKernelEx(&cfg, attention_kv8_tcgen05_kernel<true>, mq, mkv, p)
+                                                            : cudaLaunchKernelEx(&cfg, attention_kv8_tcgen05_kernel<false>, mq, mkv, p));
+    return AP_OK;
+}
+
+AP_EXPORT int ap_attention_kv8_tcgen05_status(void) {
+    int v = -1;
+    if (cudaMemcpyFromSymbol(&v, g_t8_status, sizeof(int)) != cudaSuccess) return -1;
+    return v;
+}
+
+#else   // head sizes this kernel is not built for
+
+AP_EXPORT int ap_attention_kv8_tcgen05_takes(int, int, int, int) { return 0; }
+
+#endif

@@ -44,7 +44,7 @@ CORE_SOURCES = ["errors.cu", "elementwise.cu", "gemm_simt.cu", "gemm_f32.cu", "g
                 "stream.cu", "linear_attention.cu", "postnorm.cu", "hyper_connections.cu", "kv8.cu"]
 ATTN_SOURCES = ["errors.cu", "attention.cu", "attention_tc.cu", "attention_tcgen05.cu",
                 "attention_tcgen05_wide.cu", "attention_kv8.cu",
-                "attention_kv8_decode.cu"]
+                "attention_kv8_decode.cu", "attention_kv8_tcgen05.cu"]
 HEADERS = ["common.cuh", "tcgen05.cuh", "window_bias.cuh", "gated_activation.cuh", "attention_noalloc.h", "kv8.cuh"]
 
 

@@ -835,6 +835,9 @@ def check_kernel_status() -> None:
         if hasattr(lib, "ap_attention_kv8_decode_status") and int(lib.ap_attention_kv8_decode_status()) != 0:
             raise KernelError(f"the decode attention kernel over 8-bit pages (head size {hd}) gave up waiting on its "
                               f"pipeline; its results are void")
+        if hasattr(lib, "ap_attention_kv8_tcgen05_status") and int(lib.ap_attention_kv8_tcgen05_status()) != 0:
+            raise KernelError(f"the tcgen05 attention kernel over 8-bit pages (head size {hd}) gave up waiting on its "
+                              f"pipeline; its results are void")
     lib = core()
     if hasattr(lib, "ap_gemm_tc_pair_status") and int(lib.ap_gemm_tc_pair_status()) != 0:
         raise KernelError(f"the tensor-core matrix product on pairs of SMs gave up waiting (code "

@@ -176,6 +176,35 @@ def _rows(q, out, cache_layer, block_table, token_seq, positions, first, rows, n
              page_size, float(scale), int(window), ctas, cluster, buf.data_ptr() if buf is not None else 0, need, next(_nonces) % (1 << 62) + 1, stream_handle())
 
 
+@functools.lru_cache(maxsize=None)
+def _portions_taken(num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> int:
+    """Tokens of a sequence to a CTA of the kernel for portions (0: it does not take the shape)."""
+    lib = library.attention(head_dim)
+    if not lib.ap_attention_kv8_tcgen05_takes(num_heads, num_kv_heads, head_dim, page_size):
+        return 0
+    return int(lib.ap_attention_kv8_tcgen05_tokens(num_heads, num_kv_heads))
+
+
+def plan_portions(ctas: int, tiles: int, sms: int) -> int:
+    """Key slices of the kernel for portions: ``ctas`` CTAs before slicing, rows that see up to ``tiles`` tiles of 128 keys."""
+    slices = 1
+    while slices < 8 and ctas * slices * 2 <= sms and tiles >= 4 * slices:
+        slices *= 2
+    return slices
+
+
+def _portions(q, out, cache_layer, block_table, seq_start, positions, first_seq, query_lens, T, num_heads, num_kv_heads, head_dim,
+              page_size, scale, window, per_cta, device) -> None:
+    """The sequences from ``first_seq`` on, by their ``query_lens``; their rows follow those of the sequences before."""
+    width = block_table.shape[1]
+    ctas = sum(-(-n // per_cta) for n in query_lens)
+    keys = min(width * page_size, window + per_cta) if window else width * page_size
+    call(library.attention(head_dim), "ap_attention_kv8_tcgen05", q.data_ptr(), out.data_ptr(), cache_layer.data_ptr(),
+         cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr() + 4 * first_seq * width, width,
+         seq_start.data_ptr() + 4 * first_seq, positions.data_ptr(), len(query_lens), T, num_heads, num_kv_heads, head_dim, page_size,
+         float(scale), int(window), ctas, plan_portions(ctas * num_kv_heads, -(-keys // 128), _sms(device)), stream_handle())
+
+
 def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor, block_table: torch.Tensor,
                   token_seq: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
                   page_size: int, scale: float, window: int = 0, seq_start: Optional[torch.Tensor] = None,
@@ -201,9 +230,22 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
         if seq_start.shape[0] != len(query_lens) + 1 or sum(query_lens) != T or block_table.shape[0] < len(query_lens):
             raise KernelError(f"{what}: seq_start, query_lens and the block table do not describe the rows")
     if code == AP_BF16 and T and 0 < cache_layer.numel() < 1 << 36 and _single_rows_taken(head_dim, page_size):
-        longest = max_context or block_table.shape[1] * page_size
-        _rows(q, out, cache_layer, block_table, token_seq, positions, 0, T, num_heads, num_kv_heads, head_dim, page_size, scale, window,
-              longest, min(mean_context or longest, longest), scratch, device)
+        # sequences that bring one row each, then portions (one-row sequences further back ride along with them)
+        widest = block_table.shape[1] * page_size
+        ones, rows = 0, T
+        if query_lens is not None and seq_start is not None:
+            while ones < len(query_lens) and query_lens[ones] == 1:
+                ones += 1
+            if ones < len(query_lens):
+                per_cta = _portions_taken(num_heads, num_kv_heads, head_dim, page_size) if scale > 0 else 0
+                if per_cta:
+                    _portions(q, out, cache_layer, block_table, seq_start, positions, ones, query_lens[ones:], T, num_heads,
+                              num_kv_heads, head_dim, page_size, scale, window, per_cta, device)
+                    rows = ones
+        if rows:
+            longest = max_context if max_context and rows == ones else widest
+            _rows(q, out, cache_layer, block_table, token_seq, positions, 0, rows, num_heads, num_kv_heads, head_dim, page_size, scale,
+                  window, longest, min(mean_context or longest, longest), scratch, device)
         return
     call(library.attention(head_dim), "ap_attention_kv8_rows", q.data_ptr(), out.data_ptr(), code, cache_layer.data_ptr(),
          cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr(), block_table.shape[1], block_table.shape[0],
