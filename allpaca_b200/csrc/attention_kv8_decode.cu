@@ -45,6 +45,7 @@
 #define MERGE_WARP (QUERY_WARP + 1)
 #define K8D_THREADS ((CWARPS + PWARPS + 2) * 32)
 #define MAX_STAGES 24
+#define K8D_PAIR_COST 4                        // tiles
 #define K8D_FEW_PARTS 4                        // of a pair, up to which one warp adds them up
 #define K8D_MAX_ROWS 512                       // of a launch
 // Rows lie in shared memory as TMA leaves them: `BOX` bytes to a row, the 16-byte chunks of 8 (4, 2) rows swizzled where a box is 128 (64,
@@ -121,30 +122,42 @@ struct K8dAt {
     int row, j, tile, end;                     // end: tiles of the row
 };
 
-// (W tiles, fewer than 2^31, on G CTAs: the first `more` of them take one tile beyond `each`)
+// The cuts are equal in cost: a pair costs its tiles and `pair` tiles more (its queries, its merging); the first `more` CTAs take one unit
+// beyond `each`.
 struct K8dWork {
     const int* start;                          // [T + 1] tiles before a row (shared memory)
-    int J, each, more;
-    __device__ __forceinline__ int from(int cta) const { return cta * each + min(cta, more); }
-    __device__ __forceinline__ int cta_of(int w) const {
-        const int cut = more * (each + 1);
-        return w < cut ? w / (each + 1) : more + (w - cut) / each;
-    }
-    __device__ __forceinline__ K8dAt at(int w, int T) const {
-        int lo = 0, hi = T;                    // the last row that starts at or before w
+    int T, J, pair, each, more;
+    // the row whose tiles, or costs, hold x
+    __device__ __forceinline__ int row_of(int x, int cost) const {
+        int lo = 0, hi = T;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (start[mid] * J <= w) lo = mid; else hi = mid;
+            if ((start[mid] + mid * cost) * J <= x) lo = mid; else hi = mid;
         }
+        return lo;
+    }
+    // the first tile of a CTA
+    __device__ __forceinline__ int from(int cta) const {
+        const int x = cta * each + min(cta, more), row = row_of(x, pair);
+        const int in = x - (start[row] + row * pair) * J, end = start[row + 1] - start[row];
+        const int j = min(in / (end + pair), J), rest = in - j * (end + pair);
+        return start[row] * J + j * end + min(rest, end);
+    }
+    __device__ __forceinline__ int cta_of(int w) const {
+        const int row = row_of(w, 0), end = start[row + 1] - start[row], in = w - start[row] * J, j = in / end;
+        const int x = (start[row] + row * pair) * J + in + j * pair, cut = more * (each + 1);
+        return x < cut ? x / (each + 1) : more + (x - cut) / each;
+    }
+    __device__ __forceinline__ K8dAt at(int w) const {
         K8dAt a;
-        a.row = lo;
-        a.end = start[lo + 1] - start[lo];
-        const int in = w - start[lo] * J;
+        a.row = row_of(w, 0);
+        a.end = start[a.row + 1] - start[a.row];
+        const int in = w - start[a.row] * J;
         a.j = in / a.end;
         a.tile = in - a.j * a.end;
         return a;
     }
-    __device__ __forceinline__ void next(K8dAt& a, int n, int T) const {
+    __device__ __forceinline__ void next(K8dAt& a, int n) const {
         a.tile += n;
         while (a.tile >= a.end && a.row < T) {
             a.tile -= a.end;
@@ -339,15 +352,17 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
         __syncthreads();
     }
     const int W = s_start[T] * J;
-    const int G = CL ? (int)gridDim.x : min((int)gridDim.x, W);        // without clusters: CTAs with work, so that every run holds a tile
+    const int G = CL ? (int)gridDim.x : min((int)gridDim.x, W);        // (a cut pair's parts lie in CTAs one behind the other)
     if (!CL && (int)blockIdx.x >= G) return;
-    const K8dWork work = {s_start, J, W / G, W % G};
-    const int lo = work.from(blockIdx.x), hi = work.from(blockIdx.x + 1);
+    const int pair = CL ? 0 : K8D_PAIR_COST, cost = W + T * J * pair;
+    const K8dWork work = {s_start, T, J, pair, cost / G, cost % G};
+    const int lo = work.from(blockIdx.x), hi = (int)blockIdx.x + 1 < G ? work.from(blockIdx.x + 1) : W;
+    if (!CL && lo >= hi) return;
     // The run's order: its last pair's part where the run ends inside that pair, its first pair's part where it starts inside one, then the
     // whole pairs: what has to be put together with other CTAs' parts is done while there is work left to hide it behind.
     int cut1 = CL ? hi : lo, cut2 = hi;                    // [lo, cut1) the first part, [cut1, cut2) whole pairs, [cut2, hi) the last part
     if (!CL) {
-        const K8dAt a = work.at(lo, T), b = work.at(hi - 1, T);
+        const K8dAt a = work.at(lo), b = work.at(hi - 1);
         if (a.tile) cut1 = min(hi, lo + a.end - a.tile);
         if (b.tile + 1 < b.end && hi > cut1) cut2 = hi - 1 - b.tile;
         if (cut2 < cut1) cut2 = cut1;
@@ -420,7 +435,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
             page = -1;
             krow = 0;
             if (v < tiles) {
-                const K8dAt at = work.at(place(v), T);
+                const K8dAt at = work.at(place(v));
                 const int last = s_last[at.row], first = k8d_first(p, last), tile = first / TILE + at.tile;
                 const int key0 = tile * TILE + my_page * page_rows;                        // of the page's part of the tile
                 if (key0 <= last && key0 + page_rows > first)
@@ -465,7 +480,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
         // ---- queries: of every pair ahead of its turn, split and in the order of the products' operands ----
         int k = 0;
         for (int seg = 0; seg < 3; ++seg) {
-        K8dAt at = work.at(min(run_from(seg), W - 1), T);
+        K8dAt at = work.at(min(run_from(seg), W - 1));
         for (int w = run_from(seg); w < run_to(seg); ++k) {
             const int kvh = (j0 + at.j) / p.n_chunks, chunk = j0 + at.j - kvh * p.n_chunks;
             const int head0 = kvh * group + chunk * p.heads, nheads = min(p.heads, group - chunk * p.heads);
@@ -517,7 +532,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
             if (lane == 0) tc::mbar_arrive(&q_full[k & 1]);
             w += at.end - at.tile;
             at.tile = at.end - 1;
-            work.next(at, 1, T);
+            work.next(at, 1);
         }
         }
     } else if (warp == MERGE_WARP) {
@@ -551,7 +566,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
         // (once on nothing, while the first tiles are on their way: a function's first call waits for its instructions)
         k8d_combine<NT>(merge, 0, nullptr, nullptr);
         for (int seg = 0; seg < 3; ++seg) {
-        K8dAt at = work.at(min(run_from(seg), W - 1), T);
+        K8dAt at = work.at(min(run_from(seg), W - 1));
         for (int w = run_from(seg); w < run_to(seg); ph ^= 1) {
             const int kvh = (j0 + at.j) / p.n_chunks, chunk = j0 + at.j - kvh * p.n_chunks;
             const int head0 = kvh * group + chunk * p.heads, nheads = min(p.heads, group - chunk * p.heads);
@@ -574,7 +589,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
             }
             w = item1;
             at.tile = at.end - 1;
-            work.next(at, 1, T);
+            work.next(at, 1);
         }
         }
 #pragma unroll
@@ -609,7 +624,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
     uint32_t ph = 0;
     int k = 0, v = 0, n_late = 0, late0 = 0, late1 = 0, parts0 = 0, parts1 = 0;
     for (int seg = 0; seg < 3; ++seg) {
-    K8dAt at = work.at(min(run_from(seg), W - 1), T);
+    K8dAt at = work.at(min(run_from(seg), W - 1));
     for (int w = run_from(seg); w < run_to(seg); ++k) {
         // one pair, or the part of it that is this CTA's
         const int item0 = w - at.tile, item1 = item0 + at.end, stop = item1 < hi ? item1 : hi;
@@ -682,21 +697,21 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
             }
             const int key0 = (first / TILE + tile) * TILE + half * 32;
             const bool inside = key0 >= first && key0 + 31 <= last;
-            if (!__all_sync(0xffffffffu, inside && kb[0] && kb[1] && kb[2] && kb[3])) {
+            const bool every = __all_sync(0xffffffffu, inside && kb[0] && kb[1] && kb[2] && kb[3]);
+            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+            if (!every) {
                 // keys before the first, behind the last, or without a page do not count, and what lies in the place of their values must not meet
-                // a weight of zero: it may be NaN
+                // a weight of zero: it may be NaN.  (keep0, keep1: a byte to a key of the second product's operand in this lane)
+                uint32_t keep = 0u;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int kpos = key0 - half * 32 + (i & 1 ? my_b : my_a) + (i >> 1) * 16;
                     if (kpos < first || kpos > last) kb[i] = 0u;
                     if (!kb[i]) vb[i] = 0u;
-                    if (!kb[i] && c == 0)
-#pragma unroll
-                        for (int ch = 0; ch < CHUNKS; ++ch)
-                            *reinterpret_cast<uint4*>(stage + k8_at((i & 1 ? my_b : my_a) + (i >> 1) * 16, ch, rows_shift, true)) = make_uint4(0u, 0u, 0u, 0u);
+                    keep |= kb[i] ? 0xffu << (8 * i) : 0u;
                 }
-                __syncwarp();
-                tc::fence_proxy_async();                   // (the next load into this place comes through the other proxy)
+                keep0 = __shfl_sync(0xffffffffu, keep, 4 * c);
+                keep1 = __shfl_sync(0xffffffffu, keep, 4 * c + 16);
             }
             uint32_t b0[NT], b1[NT];
 #pragma unroll
@@ -746,6 +761,10 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
                 a[1] = __byte_perm(r[0], r[1], 0x7531);
                 a[2] = __byte_perm(r[2], r[3], 0x6420);
                 a[3] = __byte_perm(r[2], r[3], 0x7531);
+                if (!every) {
+                    a[0] &= keep0; a[1] &= keep0;
+                    a[2] &= keep1; a[3] &= keep1;
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) k8_mma(o[n][i], a, b0[n], b1[n]);
             }
@@ -782,7 +801,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
             }
         }
         at.tile = at.end - 1;
-        work.next(at, 1, T);
+        work.next(at, 1);
     }
     }
     // pairs of many parts: where all are there, bring them, this warp every CWARPS-th
@@ -882,7 +901,7 @@ AP_EXPORT int ap_attention_kv8_decode(const void* q, void* out, const void* cach
     AP_REQUIRE(cluster || ((uintptr_t)scratch & 15) == 0 && scratch && scratch_bytes >= ap_attention_kv8_decode_scratch(nh, nkv, ctas),
                "attention_kv8: %lld bytes of scratch are too few", scratch_bytes);
     const int heads = k8d_heads(nh, nkv), chunks = (nh / nkv + heads - 1) / heads;
-    AP_REQUIRE((long long)T * nkv * chunks * ((long long)max_blocks * P / TILE + 2) < (1LL << 31),
+    AP_REQUIRE((long long)T * nkv * chunks * ((long long)max_blocks * P / TILE + 2 + K8D_PAIR_COST) < (1LL << 31),
                "attention_kv8: %d rows over block tables of %d pages are more than 2^31 tiles", T, max_blocks);
     if (T == 0) return AP_OK;
     K8dParams p;
