@@ -1,18 +1,17 @@
 // Causal grouped-query attention of portions over the 8-bit paged cache (kv8.cuh) on the 5th-generation tensor cores, for head sizes
 // 64 and 128 (-DAP_HEAD_DIM): sequences that bring several new rows each, from two on, packed one behind the other.
 //
-// The arithmetic is that of attention_tcgen05_wide.cu: a CTA owns up to 256 rows, two tiles "a" and "b" of (128 / group) tokens x the
+// Two kernels.  The first widens the keys that the step's rows see, once: c * 2^e, exact in bfloat16, from pages into dense rows of
+// scratch memory, a sequence's keys of one KV head one behind the other; what lies outside, or has no page, becomes zeros.  The
+// second has the arithmetic of attention_tcgen05_wide.cu: a CTA owns up to 256 rows, two tiles "a" and "b" of (128 / group) tokens x the
 // `group` query heads of one KV head, and every tile of 128 keys serves both; S and O live in tensor memory, the two tiles take turns
 // on the tensor cores while the other's softmax warps work (one row to a thread, P in bfloat16 over the S it came from, O scaled
-// down only when a row's maximum has grown by more than 2^8 over its reference).
+// down only when a row's maximum has grown by more than 2^8 over its reference).  Its loads are one box to half a tile.
 //
-// What is different is where K and V come from.  A loading warp brings the 8-bit numbers and the scale bytes of a tile's keys, or
-// values, into one of two raw buffers (TMA, a box to a page; 16 KB, half of what bfloat16 pages would move), and four more warps
-// turn them into the bfloat16 tiles that the products read: c * 2^e, exact, as scales are powers of two.  So nothing else changes, and no
-// precision is lost against a bfloat16 cache that holds the same values.  Per 16 numbers that is one 16-byte load, 40 conversions and
-// multiplications, two 16-byte stores, in an order that meets no bank twice (two rows to eight lanes); against the products'
-// 2750 cycles and more to a key tile of both query tiles it takes some 1000 of the issue slots of each scheduler.  Keys outside the range
-// that the CTA's rows see, and keys without a page, become zeros: what lies in their place may be NaN.
+// Widening first costs 6 bytes of traffic to a number, half of it in L2 where the keys fit there.  Widening inside the second kernel, every
+// tile in every CTA that reads it, was built and measured: four to six warps needed 3400 to 5100 cycles to a key tile, loading a box to
+// a page 4400, where the products and the softmax need 3700: 1470 us for 2048 rows behind 30000 keys (1.2 TFLOP), the two
+// kernels KV8_BIG; 17 rows behind 8191 keys 39 us, the two kernels KV8_FEW.
 //
 // Few rows leave most SMs idle: then the keys are cut into slices, a cluster of 2, 4 or 8 CTAs works on one set of rows, and the slices'
 // sums are added up through distributed shared memory, every CTA taking its share of the rows.  One launch, no scratch.
@@ -38,11 +37,10 @@
 #define SUB_BYTES (128 * 128)              // a [128 rows x 64 bf16] sub-tile
 #define Q_BYTES (NHALF * SUB_BYTES)        // one query tile
 #define KV_BYTES (NHALF * SUB_BYTES)       // K (or V) of one tile
-#define RAW_BYTES (BKV * HD)               // the same in 8 bits
-#define T8_THREADS 512                     // 2 x 4 softmax warps; loading warp, MMA warp, two idle ones; four converting warps
+#define T8_STAGES 2
+#define T8_THREADS 384                     // 2 x 4 softmax warps; loading warp, MMA warp, two idle ones
 #define T8_LOAD_WARP 8
 #define T8_MMA_WARP 9
-#define T8_CONVERT_WARP 12
 #define T8_TMEM_COLS 512                   // S_a, S_b: 2 x 128 columns; O_a, O_b: 2 x HD
 #define T8_O_COL 256
 #define T8_PITCH (HD + 4)                  // a row of sums that slices exchange, in floats
@@ -65,30 +63,87 @@ __device__ __forceinline__ float t8_exp2(float x) {
 
 struct AttnT8Params {
     bf16* out;
-    const uint8_t* cache;
     const int* block_table;
     const int* seq_start;
     const int* positions;
-    size_t page_bytes;
     int num_pages, max_blocks, nseq, nh, nkv, P, window, group, tokens_per_tile;   // tokens_per_tile: of one query tile
-    int nsplit;
+    int nsplit, cap;                                      // cap: dense rows of a sequence's keys in one KV head, whole tiles
     float scale_log2;
 };
+
+// What the rows of sequence s see: tiles t_lo .. t_hi of its keys (none: t_hi < t_lo), keys kmin .. kmax
+__device__ __forceinline__ void t8_span(const int* positions, int row0, int ntok, int window, int last_key, int& kmin, int& kmax) {
+    kmax = min(positions[row0 + ntok - 1], last_key);
+    const int first = positions[row0];
+    kmin = (window > 0 && first - window + 1 > 0) ? first - window + 1 : 0;
+}
+
+// ---- widening: grid (tiles of a sequence's keys, keys and values of every KV head, sequences) ----
+#define T8_WIDEN_THREADS 256
+__global__ void __launch_bounds__(T8_WIDEN_THREADS)
+kv8_widen_kernel(const uint8_t* __restrict__ cache, size_t page_bytes, const AttnT8Params p, bf16* __restrict__ dense) {
+    __shared__ long long at_s[BKV];                       // where a key's numbers lie (-1: nowhere)
+    __shared__ float scale_s[BKV];
+    const int s = blockIdx.z, plane = blockIdx.y, t = blockIdx.x;
+    ap_pdl_trigger();
+    ap_pdl_wait();
+    const int row0 = p.seq_start[s], ntok = p.seq_start[s + 1] - row0;
+    if (ntok <= 0) return;
+    int kmin, kmax;
+    t8_span(p.positions, row0, ntok, p.window, p.max_blocks * p.P - 1, kmin, kmax);
+    if (kmax < 0 ? t > 0 : (t < kmin / BKV || t > kmax / BKV)) return;      // (rows that see nothing still multiply one tile)
+    if (threadIdx.x < BKV) {
+        const int kpos = t * BKV + threadIdx.x;
+        long long at = -1;
+        float scale = 0.f;
+        if (kpos >= kmin && kpos <= kmax) {
+            const int page = p.block_table[(size_t)s * p.max_blocks + kpos / p.P];
+            if (page >= 0 && page < p.num_pages) {
+                const size_t row = (size_t)plane * p.P + kpos % p.P;
+                at = (long long)((size_t)page * page_bytes + row * HD);
+                scale = kv8_scale(cache[(size_t)page * page_bytes + (size_t)2 * p.nkv * p.P * HD + row]);
+            }
+        }
+        at_s[threadIdx.x] = at;
+        scale_s[threadIdx.x] = scale;
+    }
+    __syncthreads();
+    // eight numbers to a thread and turn: whole rows of 8-byte loads and 16-byte stores side by side
+    bf16* to = dense + (((size_t)s * 2 * p.nkv + plane) * p.cap + (size_t)t * BKV) * HD;
+    constexpr int kItems = BKV * HD / 8 / T8_WIDEN_THREADS;
+    uint2 u[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int e = i * T8_WIDEN_THREADS + threadIdx.x, r = e / (HD / 8);
+        const long long at = at_s[r];
+        u[i] = at >= 0 ? *reinterpret_cast<const uint2*>(cache + at + (e - r * (HD / 8)) * 8) : make_uint2(0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int e = i * T8_WIDEN_THREADS + threadIdx.x, r = e / (HD / 8);
+        const float f = scale_s[r];
+        const float4 a = kv8_unpack(u[i].x), b = kv8_unpack(u[i].y);
+        uint4 o;
+        __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&o);
+        o2[0] = __floats2bfloat162_rn(a.x * f, a.y * f);
+        o2[1] = __floats2bfloat162_rn(a.z * f, a.w * f);
+        o2[2] = __floats2bfloat162_rn(b.x * f, b.y * f);
+        o2[3] = __floats2bfloat162_rn(b.z * f, b.w * f);
+        *reinterpret_cast<uint4*>(to + (size_t)e * 8) = o;
+    }
+}
 
 struct T8Smem {
     static constexpr int kQ = 0;                                  // tile a, tile b
     static constexpr int kK = kQ + 2 * Q_BYTES;
-    static constexpr int kV = kK + 2 * KV_BYTES;
-    static constexpr int kRaw = kV + 2 * KV_BYTES;                // two buffers
-    static constexpr int kScale = kRaw + 2 * RAW_BYTES;           // their scale bytes
-    static constexpr int kBars = kScale + 2 * BKV;
+    static constexpr int kV = kK + T8_STAGES * KV_BYTES;
+    static constexpr int kBars = kV + T8_STAGES * KV_BYTES;
     static constexpr int kTotal = kBars + 256 + 1024;             // + alignment slack
     // slices: [row of both tiles][T8_PITCH], then [row][maximum, sum], over Q, K and V when all is done
     static constexpr int kSums = 0;
     static constexpr int kStats = 2 * BQ * T8_PITCH * 4;
 };
-static_assert(T8Smem::kStats + 2 * BQ * 8 <= T8Smem::kRaw, "the slices' sums lie over the tiles");
-static_assert(T8Smem::kTotal <= 227 * 1024, "shared memory");
+static_assert(T8Smem::kStats + 2 * BQ * 8 <= T8Smem::kBars, "the slices' sums lie over the tiles");
 
 template <bool SPLIT>
 __global__ void __launch_bounds__(T8_THREADS, 1)
@@ -98,9 +153,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = (uint64_t*)(smem + T8Smem::kBars);
     uint64_t* q_full = bars + 0;
-    uint64_t* raw_full = bars + 1;                        // [buffer]
-    uint64_t* raw_free = raw_full + 2;                    // [buffer]
-    uint64_t* k_full = raw_free + 2;                      // [stage]
+    uint64_t* k_full = bars + 1;                          // [stage]
     uint64_t* v_full = k_full + 2;                        // [stage]
     uint64_t* kv_free = v_full + 2;                       // [key tile & 1]: V of that tile and K of the next are read
     uint64_t* s_full = kv_free + 2;                       // [query tile]
@@ -128,10 +181,8 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         *s_tile = t;
         tc::mbar_init(q_full, 1);
         for (int x = 0; x < 2; ++x) {
-            tc::mbar_init(&raw_full[x], 1 + 32);          // what TMA brings, and the lanes' scale bytes
-            tc::mbar_init(&raw_free[x], 4);
-            tc::mbar_init(&k_full[x], 4);
-            tc::mbar_init(&v_full[x], 4);
+            tc::mbar_init(&k_full[x], 1);
+            tc::mbar_init(&v_full[x], 1);
             tc::mbar_init(&kv_free[x], 1);
             tc::mbar_init(&s_full[x], 1);
             tc::mbar_init(&p_ready[x], 4);                // one arrival per warp of the tile's group
@@ -166,9 +217,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     const bool has_b = ntok > p.tokens_per_tile;          // the second query tile holds rows
     ap_pdl_wait();
     if (active) {
-        kmax = min(p.positions[row0 + ntok - 1], p.max_blocks * p.P - 1);
-        const int first = p.positions[row0];
-        kmin = (p.window > 0 && first - p.window + 1 > 0) ? first - p.window + 1 : 0;
+        t8_span(p.positions, row0, ntok, p.window, p.max_blocks * p.P - 1, kmin, kmax);
     }
     int t_lo = kmin / BKV, t_hi = active ? kmax / BKV : -1;
     if (SPLIT) {
@@ -178,27 +227,19 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     }
     const int ntiles = max(t_hi - t_lo + 1, 0);
     const int* table = p.block_table + (size_t)(active ? seq : 0) * p.max_blocks;
-    const int n_pages = p.P < BKV ? BKV / p.P : 1, page_rows = BKV / n_pages;      // of a tile
-    // the page of lane `lane` of tile `it` (-1: none)
+    // The pages of a tile's keys, one to a lane (a page larger than a tile: lane 0's), are looked at only to know which are not there
+    const int page_rows = min(p.P, BKV), n_pages = BKV / page_rows;
     auto page_of = [&](int it) {
         const int key0 = (t_lo + it) * BKV + lane * page_rows;
-        if (it >= ntiles || lane >= n_pages || key0 > kmax || key0 + page_rows - 1 < kmin) return -1;
+        if (it >= ntiles || lane >= n_pages || key0 > kmax || key0 + page_rows - 1 < kmin) return 0;
         const int page = table[key0 / p.P];
         return page < p.num_pages ? page : -1;
     };
-    // Tiles go K 0, K 1, V 0, K 2, V 1, ...: K runs one tile ahead of V.  The n-th of them:
-    auto nth = [&](int n, int& it, int& which) {
-        if (n == 0) { it = 0; which = 0; return; }
-        if (ntiles == 1) { it = 0; which = 1; return; }
-        if (n == 2 * ntiles - 1) { it = ntiles - 1; which = 1; return; }
-        it = (n & 1) ? (n + 1) / 2 : n / 2 - 1;
-        which = (n & 1) ? 0 : 1;
-    };
 
-    // Registers move from the warps that issue and convert to the softmax warps, which hold a row of 128 scores each (the unit of such a
-    // move is four warps): 2 x 192 + 64 + 64 = 512 to a thread of each, what the launch holds.
-    if (warp >= 8 && warp < T8_CONVERT_WARP) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    // Registers move from the warps that only issue copies and products to the softmax warps, which hold a row of 128 scores each (the
+    // unit of such a move is four warps): 2 x 224 + 56 = 504 to a thread of each, what the launch holds.
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == T8_LOAD_WARP) {
         if (active && ntiles > 0) {
             if (lane == 0) {
@@ -207,49 +248,29 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                     for (int h = 0; h < NHALF; ++h)
                         tc::tma_load_3d(smem + T8Smem::kQ + x * Q_BYTES + h * SUB_BYTES, &tmap_q, h * 64, head0,
                                         row0 + x * p.tokens_per_tile, q_full);
-            }
-            const int s_page = lane * 4 / page_rows;       // the page of this lane's four scale bytes
-            const uint8_t* const scales = p.cache + (size_t)2 * p.nkv * p.P * HD + (lane * 4 & (page_rows - 1));
-            int n = 0;
-            auto load = [&](int it, int which, int page) -> bool {
-                const int b = n & 1;
-                const int there = __popc(__ballot_sync(0xffffffffu, page >= 0));
-                const int page_s = __shfl_sync(0xffffffffu, page, s_page);
-                int fine = 1;
-                if (lane == 0) {
-                    if (*abort_flag) fine = 0;
-                    if (fine && !tc::mbar_wait(&raw_free[b], (uint32_t)((n >> 1) & 1) ^ 1)) {
+                const int k_row = (seq * 2 * p.nkv + kvh) * p.cap + t_lo * BKV, v_row = k_row + p.nkv * p.cap;
+                // `after`: the key tile whose turn in the MMA warp frees the stage (kv_free is given one arrival before the first
+                // turn, "tile -1", and one at the end of every turn): K of tile j - 2 was read in turn j - 3, V of it in turn j - 2
+                auto load = [&](int it, int row, uint64_t* full, int after, int base) -> bool {
+                    const int s = it % T8_STAGES;
+                    if (*abort_flag) return false;
+                    if (it >= T8_STAGES && !tc::mbar_wait(&kv_free[after & 1], (uint32_t)(((after + (after & 1)) >> 1) & 1))) {
                         *abort_flag = 1;
                         atomicExch(&g_t8_status, T8_ERR_WAIT);
-                        fine = 0;
+                        return false;
                     }
-                    if (fine) tc::mbar_expect_tx(&raw_full[b], (uint32_t)(there * page_rows * HD));
+                    tc::mbar_expect_tx(&full[s], KV_BYTES);
+                    for (int h = 0; h < NHALF; ++h)
+                        tc::tma_load_2d(smem + base + s * KV_BYTES + h * SUB_BYTES, &tmap_kv, h * 64, row + it * BKV, &full[s]);
+                    return true;
+                };
+                // K runs one tile ahead of V
+                bool fine = load(0, k_row, k_full, 0, T8Smem::kK);
+                for (int it = 0; it < ntiles && fine; ++it) {
+                    if (it + 1 < ntiles) fine = load(it + 1, k_row, k_full, it - 2, T8Smem::kK);
+                    if (fine) fine = load(it, v_row, v_full, it - 2, T8Smem::kV);
                 }
-                fine = __shfl_sync(0xffffffffu, fine, 0);
-                if (!fine) return false;
-                const int krow = (which * p.nkv + kvh) * p.P + (p.P > BKV ? (t_lo + it) * BKV % p.P : 0);
-                if (page >= 0)
-                    tc::tma_load_3d(smem + T8Smem::kRaw + b * RAW_BYTES + lane * page_rows * HD, &tmap_kv, 0, krow, page, &raw_full[b]);
-                const uint8_t* sc = scales + (size_t)max(page_s, 0) * p.page_bytes + krow;
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(tc::smem_addr(smem + T8Smem::kScale + b * BKV + lane * 4)),
-                             "l"(sc), "r"(page_s >= 0 ? 4 : 0) : "memory");
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(tc::smem_addr(&raw_full[b])) : "memory");
-                ++n;
-                return true;
-            };
-            // K runs one tile ahead of V; the block table is read four tiles ahead of its use
-            int page_v = page_of(0);
-            int q0 = page_of(1), q1 = page_of(2), q2 = page_of(3), q3 = page_of(4);
-            bool fine = load(0, 0, page_v);
-            for (int it = 0; it < ntiles && fine; ++it) {
-                const int page_k = q0;
-                q0 = q1; q1 = q2; q2 = q3;
-                q3 = page_of(it + 5);
-                if (it + 1 < ntiles) fine = load(it + 1, 0, page_k);
-                if (fine) fine = load(it, 1, page_v);
-                page_v = page_k;
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     } else if (warp == T8_MMA_WARP) {
         if (lane == 0 && active && ntiles > 0) {
@@ -306,67 +327,8 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             }
         }
     }
-    } else if (warp >= T8_CONVERT_WARP) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    if (active && ntiles > 0) {
-        // Lane l of sixteen takes 16-byte chunk l & 7 (head size 64: l & 3) of one of two rows: eight lanes read 128 bytes in a row, and what
-        // they write, even chunks of the one row and odd ones of the other, lies in different banks.
-        const int cw = warp - T8_CONVERT_WARP;
-        const int q = HD == 128 ? lane & 7 : lane & 3;
-        const int r2 = HD == 128 ? (lane >> 4) * 2 + (((lane >> 2) ^ (lane >> 3)) & 1) : lane >> 2;     // of the 4 (8) rows of a warp's run
-        constexpr int kRows = HD == 128 ? 4 : 8;
-        bool ok = true;
-        for (int n = 0; n < 2 * ntiles && ok; ++n) {
-            int it, which;
-            nth(n, it, which);
-            const int b = n & 1, s = it & 1;
-            ok = __all_sync(0xffffffffu, tc::mbar_wait(&raw_full[b], (uint32_t)((n >> 1) & 1)));
-            // the stage's last readers: K of tile j - 2 in turn j - 3, V of tile j - 2 in turn j - 2 (kv_free is given one arrival
-            // before the first turn, "tile -1", and one at the end of every turn)
-            const int after = which ? it - 2 : it - 3;
-            if (ok && it >= 2) ok = __all_sync(0xffffffffu, tc::mbar_wait(&kv_free[after & 1], (uint32_t)(((after + (after & 1)) >> 1) & 1)));
-            if (!ok) {
-                if (!*abort_flag) {
-                    *abort_flag = 1;
-                    atomicExch(&g_t8_status, T8_ERR_WAIT);
-                }
-                break;
-            }
-            const uint8_t* raw = smem + T8Smem::kRaw + b * RAW_BYTES;
-            const uint8_t* scale = smem + T8Smem::kScale + b * BKV;
-            uint8_t* to = smem + (which ? T8Smem::kV : T8Smem::kK) + s * KV_BYTES + (q >> 2) * SUB_BYTES;
-            const int key0 = (t_lo + it) * BKV;
-#pragma unroll 4
-            for (int i = 0; i < BKV / (4 * kRows); ++i) {
-                const int r = (i * 4 + cw) * kRows + r2;
-                const uint4 u = *reinterpret_cast<const uint4*>(raw + r * HD + q * 16);
-                const uint32_t byte = scale[r];
-                const bool is = byte != 0 && key0 + r >= kmin && key0 + r <= kmax;
-                const float2 f2 = make_float2(kv8_scale(byte), kv8_scale(byte));
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-                uint32_t o[8];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float4 f = kv8_unpack(w[k]);
-                    const float2 lo = __fmul2_rn(make_float2(f.x, f.y), f2), hi = __fmul2_rn(make_float2(f.z, f.w), f2);
-                    __nv_bfloat162 a = __floats2bfloat162_rn(lo.x, lo.y), c = __floats2bfloat162_rn(hi.x, hi.y);
-                    o[2 * k] = is ? *reinterpret_cast<uint32_t*>(&a) : 0u;
-                    o[2 * k + 1] = is ? *reinterpret_cast<uint32_t*>(&c) : 0u;
-                }
-                const int c0 = (q & 3) * 2;
-                *reinterpret_cast<uint4*>(to + r * 128 + ((c0 ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<uint4*>(to + r * 128 + (((c0 + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-            }
-            tc::fence_proxy_async();                       // the products read through the other proxy
-            __syncwarp();
-            if (lane == 0) {
-                tc::mbar_arrive(&raw_free[b]);
-                tc::mbar_arrive(which ? &v_full[s] : &k_full[s]);
-            }
-        }
-    }
     } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     if (active && (warp < 4 || has_b)) {
         // ---- softmax: warps 0..3 own query tile a, warps 4..7 tile b; one row per thread ----
         const int x = warp >> 2;
@@ -383,14 +345,14 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         int page = page_of(0);
         for (int it = 0; it < ntiles; ++it) {
             const int k0 = (t_lo + it) * BKV;
-            // pages that the rows' keys lie in and that are not there (rare: a caller gives them back behind a window only)
-            const int mine = k0 + lane * page_rows;
-            const uint32_t gone = __ballot_sync(0xffffffffu, lane < n_pages && page < 0 && mine <= kmax && mine + page_rows - 1 >= kmin);
+            // pages that are not there (rare: a caller gives them back behind a window)
+            const uint32_t gone = __ballot_sync(0xffffffffu, page < 0);
             page = page_of(it + 1);
             // tcgen05.ld and .st are warp-wide instructions: whatever decides whether one runs is a vote
             if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_full[x], (uint32_t)(it & 1)))) { ok = false; break; }
             tc::fence_after_sync();
-            const bool row_all = rvalid && k0 + BKV - 1 <= qpos && (p.window <= 0 || qpos - k0 < p.window);
+            // (rows that are none see everything: their sums go nowhere)
+            const bool row_all = !rvalid || (k0 + BKV - 1 <= qpos && (p.window <= 0 || qpos - k0 < p.window));
             const bool row_none = !rvalid || k0 > qpos || (p.window > 0 && qpos - (k0 + BKV - 1) >= p.window);
             const bool all_visible = __all_sync(0xffffffffu, row_all) && gone == 0;
             const bool none_visible = __all_sync(0xffffffffu, row_none);
@@ -412,7 +374,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
 #pragma unroll
                     for (int j = 0; j < 128; ++j) {
                         const int kpos = k0 + j;
-                        const bool vis = rvalid && kpos <= qpos && (p.window <= 0 || qpos - kpos < p.window);
+                        const bool vis = kpos <= qpos && (p.window <= 0 || qpos - kpos < p.window);
                         v[j] = vis ? v[j] : 0xff800000u;
                     }
                     if (gone != 0) {
@@ -594,27 +556,37 @@ AP_EXPORT int ap_attention_kv8_tcgen05_takes(int nh, int nkv, int hd, int P) {
     if (hd != HD || nkv <= 0 || nh % nkv) return 0;
     const int g = nh / nkv;
     if (g > 128 || 128 % g) return 0;
-    if (P < 8 || (P < BKV ? BKV % P : (P % BKV || P > 65536))) return 0;
+    if (P < 8 || (P < BKV ? BKV % P : P % BKV)) return 0;
     return t8_encode_fn() != nullptr;
 }
 
 // tokens of one sequence that one CTA takes (two query tiles)
 AP_EXPORT int ap_attention_kv8_tcgen05_tokens(int nh, int nkv) { return 2 * (128 / (nh / nkv)); }
 
-// q: [T][nh][HD]; total_ctas: the sum over the sequences of ceil(rows / tokens of a CTA); nsplit: 1, 2, 4 or 8 key slices; scale > 0.
+// Bytes of scratch for `nseq` sequences with block tables of `max_blocks` pages
+AP_EXPORT long long ap_attention_kv8_tcgen05_scratch(int nseq, int max_blocks, int P, int nkv) {
+    return 2LL * nseq * 2 * nkv * (((long long)max_blocks * P + BKV - 1) / BKV * BKV) * HD;
+}
+
+// q: [T][nh][HD]; total_ctas: the sum over the sequences of ceil(rows / tokens of a CTA); nsplit: 1, 2, 4 or 8 key slices; scale > 0;
+// scratch: ap_attention_kv8_tcgen05_scratch bytes of any contents, 16-byte aligned, of no call that runs at the same time.
 AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cache, long long num_pages, long long page_bytes,
                                        const int* block_table, int max_blocks, const int* seq_start, const int* positions, int nseq, int T,
-                                       int nh, int nkv, int hd, int P, float scale, int window, int total_ctas, int nsplit,
-                                       cudaStream_t stream) {
+                                       int nh, int nkv, int hd, int P, float scale, int window, int total_ctas, int nsplit, void* scratch,
+                                       long long scratch_bytes, cudaStream_t stream) {
     AP_REQUIRE(ap_attention_kv8_tcgen05_takes(nh, nkv, hd, P), "attention_kv8 (tcgen05): shape not supported: heads=%d kv_heads=%d "
                "head_dim=%d page=%d", nh, nkv, hd, P);
     AP_REQUIRE(T > 0 && nseq > 0 && total_ctas > 0 && max_blocks > 0, "attention_kv8 (tcgen05): bad sizes");
-    AP_REQUIRE(num_pages > 0 && num_pages < (1LL << 31) && page_bytes == kv8_page_bytes(nkv, P, HD), "attention_kv8: the pages do not match the heads");
-    AP_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)cache & 15) == 0 && ((uintptr_t)out & 15) == 0,
+    AP_REQUIRE(num_pages >= 0 && num_pages < (1LL << 31) && page_bytes == kv8_page_bytes(nkv, P, HD), "attention_kv8: the pages do not match the heads");
+    AP_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)cache & 15) == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)scratch & 15) == 0,
                "attention_kv8 (tcgen05): operands must be 16-byte aligned");
-    AP_REQUIRE((long long)max_blocks * P < (1LL << 31) - 256, "attention_kv8: the block table names more than 2^31 keys");
+    const long long cap = ((long long)max_blocks * P + BKV - 1) / BKV * BKV, dense_rows = (long long)nseq * 2 * nkv * cap;
+    AP_REQUIRE(dense_rows < (1LL << 31) - 256, "attention_kv8 (tcgen05): %lld rows of keys and values are too many", dense_rows);
+    AP_REQUIRE(scratch && scratch_bytes >= ap_attention_kv8_tcgen05_scratch(nseq, max_blocks, P, nkv), "attention_kv8 (tcgen05): %lld bytes of "
+               "scratch are too few", scratch_bytes);
     AP_REQUIRE(scale > 0.f, "attention_kv8 (tcgen05): the scale must be positive");
     AP_REQUIRE(nsplit == 1 || nsplit == 2 || nsplit == 4 || nsplit == 8, "attention_kv8: bad number of key slices %d", nsplit);
+    AP_REQUIRE(nseq <= 65535 && 2 * nkv <= 65535, "attention_kv8 (tcgen05): %d sequences of %d KV heads exceed the grid", nseq, nkv);
     const int G = nh / nkv;
     CUtensorMap mq, mkv;
     {
@@ -628,15 +600,14 @@ AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cac
                    "attention_kv8 (tcgen05): cannot encode the query tensor map");
     }
     {
-        // [page][keys and values: head and row][number]; a box is one page's rows of one head
-        cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)2 * nkv * P, (cuuint64_t)num_pages};
-        cuuint64_t strides[2] = {(cuuint64_t)HD, (cuuint64_t)page_bytes};
-        cuuint32_t box[3] = {HD, (cuuint32_t)(P < BKV ? P : BKV), 1};
-        cuuint32_t es[3] = {1, 1, 1};
-        AP_REQUIRE(t8_encode_fn()(&mkv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(cache), dims, strides, box, es,
-                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)dense_rows};
+        cuuint64_t strides[1] = {(cuuint64_t)HD * 2};
+        cuuint32_t box[2] = {64, BKV};
+        cuuint32_t es[2] = {1, 1};
+        AP_REQUIRE(t8_encode_fn()(&mkv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, scratch, dims, strides, box, es,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS,
-                   "attention_kv8 (tcgen05): cannot encode the cache tensor map");
+                   "attention_kv8 (tcgen05): cannot encode the tensor map of keys and values");
     }
     static bool configured[64];
     int dev = 0;
@@ -650,11 +621,13 @@ AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cac
         configured[dev] = true;
     }
     AttnT8Params p;
-    p.out = (bf16*)out; p.cache = (const uint8_t*)cache; p.block_table = block_table; p.seq_start = seq_start; p.positions = positions;
-    p.page_bytes = (size_t)page_bytes; p.num_pages = (int)num_pages; p.max_blocks = max_blocks; p.nseq = nseq; p.nh = nh; p.nkv = nkv;
+    p.out = (bf16*)out; p.block_table = block_table; p.seq_start = seq_start; p.positions = positions;
+    p.cap = (int)cap; p.num_pages = (int)num_pages; p.max_blocks = max_blocks; p.nseq = nseq; p.nh = nh; p.nkv = nkv;
     p.P = P; p.window = window; p.group = G; p.tokens_per_tile = 128 / G; p.nsplit = nsplit;
     p.scale_log2 = scale * LOG2E_F;
     AP_REQUIRE((long long)total_ctas * nkv < (1LL << 31), "attention_kv8 (tcgen05): too many CTAs for the grid");
+    AP_CHECK_PDL_LAUNCH("kv8_widen", ap_launch_pdl(kv8_widen_kernel, dim3((unsigned)(cap / BKV), 2 * nkv, nseq), dim3(T8_WIDEN_THREADS), 0, stream,
+                                                     (const uint8_t*)cache, (size_t)page_bytes, p, (bf16*)scratch));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(total_ctas * nkv), nsplit);
     cfg.blockDim = dim3(T8_THREADS);

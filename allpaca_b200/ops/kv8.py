@@ -193,16 +193,28 @@ def plan_portions(ctas: int, tiles: int, sms: int) -> int:
     return slices
 
 
+# bytes of scratch for widened keys and values up to which sequences go together
+WIDE_SCRATCH = 1 << 30
+
+
 def _portions(q, out, cache_layer, block_table, seq_start, positions, first_seq, query_lens, T, num_heads, num_kv_heads, head_dim,
-              page_size, scale, window, per_cta, device) -> None:
+              page_size, scale, window, per_cta, scratch, device) -> None:
     """The sequences from ``first_seq`` on, by their ``query_lens``; their rows follow those of the sequences before."""
-    width = block_table.shape[1]
-    ctas = sum(-(-n // per_cta) for n in query_lens)
+    width, lib = block_table.shape[1], library.attention(head_dim)
+    one = lib.ap_attention_kv8_tcgen05_scratch(1, width, page_size, num_kv_heads)
+    step = max(1, min(len(query_lens), WIDE_SCRATCH // one))
+    buf = scratch("attn.kv8_wide", (step * one // 2,), torch.bfloat16) if scratch is not None else \
+        torch.empty(step * one // 2, dtype=torch.bfloat16, device=q.device)
     keys = min(width * page_size, window + per_cta) if window else width * page_size
-    call(library.attention(head_dim), "ap_attention_kv8_tcgen05", q.data_ptr(), out.data_ptr(), cache_layer.data_ptr(),
-         cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr() + 4 * first_seq * width, width,
-         seq_start.data_ptr() + 4 * first_seq, positions.data_ptr(), len(query_lens), T, num_heads, num_kv_heads, head_dim, page_size,
-         float(scale), int(window), ctas, plan_portions(ctas * num_kv_heads, -(-keys // 128), _sms(device)), stream_handle())
+    for at in range(0, len(query_lens), step):
+        n = min(step, len(query_lens) - at)
+        ctas = sum(-(-rows // per_cta) for rows in query_lens[at:at + n])
+        if ctas:
+            call(lib, "ap_attention_kv8_tcgen05", q.data_ptr(), out.data_ptr(), cache_layer.data_ptr(), cache_layer.shape[0],
+                 cache_layer.shape[1], block_table.data_ptr() + 4 * (first_seq + at) * width, width,
+                 seq_start.data_ptr() + 4 * (first_seq + at), positions.data_ptr(), n, T, num_heads, num_kv_heads, head_dim, page_size,
+                 float(scale), int(window), ctas, plan_portions(ctas * num_kv_heads, -(-keys // 128), _sms(device)), buf.data_ptr(),
+                 step * one, stream_handle())
 
 
 def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor, block_table: torch.Tensor,
@@ -240,7 +252,7 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
                 per_cta = _portions_taken(num_heads, num_kv_heads, head_dim, page_size) if scale > 0 else 0
                 if per_cta:
                     _portions(q, out, cache_layer, block_table, seq_start, positions, ones, query_lens[ones:], T, num_heads,
-                              num_kv_heads, head_dim, page_size, scale, window, per_cta, device)
+                              num_kv_heads, head_dim, page_size, scale, window, per_cta, scratch, device)
                     rows = ones
         if rows:
             longest = max_context if max_context and rows == ones else widest

@@ -283,6 +283,7 @@ def test_portions_on_tensor_cores(ops, slices, nh, nkv, hd, P, window, monkeypat
     """Portions of two rows to several CTAs' worth, key slices that hold many tiles, one or none, one-row sequences among them."""
     from allpaca_b200.ops import kv8
     monkeypatch.setattr(kv8, "plan_portions", lambda *a: slices)
+    monkeypatch.setattr(kv8, "WIDE_SCRATCH", (1 << 30) if slices < 4 else 1)          # all sequences together, or one by one
     for seqs in ([(1500, 2), (700, 70), (129, 129), (1, 1), (64, 1), (2, 2), (3000, 300)], [(130, 130)], [(257, 2)]):
         c = plain.case(seqs, nh, nkv, hd, P, torch.bfloat16, seed=slices + hd)
         check(run(ops, c, 0.09, window), c, 0.09, window)
