@@ -11,7 +11,7 @@
 // Widening first costs 6 bytes of traffic to a number, half of it in L2 where the keys fit there.  Widening inside the second kernel, every
 // tile in every CTA that reads it, was built and measured: four to six warps needed 3400 to 5100 cycles to a key tile, loading a box to
 // a page 4400, where the products and the softmax need 3700: 1470 us for 2048 rows behind 30000 keys (1.2 TFLOP), the two
-// kernels KV8_BIG; 17 rows behind 8191 keys 39 us, the two kernels KV8_FEW.
+// kernels 1015; 17 rows behind 8191 keys 39 us, the two kernels 37.
 //
 // Few rows leave most SMs idle: then the keys are cut into slices, a cluster of 2, 4 or 8 CTAs works on one set of rows, and the slices'
 // sums are added up through distributed shared memory, every CTA taking its share of the rows.  One launch, no scratch.
@@ -37,12 +37,12 @@
 #define SUB_BYTES (128 * 128)              // a [128 rows x 64 bf16] sub-tile
 #define Q_BYTES (NHALF * SUB_BYTES)        // one query tile
 #define KV_BYTES (NHALF * SUB_BYTES)       // K (or V) of one tile
-#define T8_STAGES 2
-#define T8_THREADS 384                     // 2 x 4 softmax warps; loading warp, MMA warp, two idle ones
-#define T8_LOAD_WARP 8
-#define T8_MMA_WARP 9
-#define T8_TMEM_COLS 512                   // S_a, S_b: 2 x 128 columns; O_a, O_b: 2 x HD
-#define T8_O_COL 256
+// One query tile (NX = 1) or two to a CTA: threads (four softmax warps to a tile; loading warp, MMA warp, two idle ones), stages of K and V,
+// columns of tensor memory (S: 128 to a tile, O: HD)
+#define T8_THREADS(NX) ((NX) * 128 + 128)
+#define T8_STAGES(NX) (NX)
+#define T8_TMEM_COLS(NX) ((NX) * 256)
+#define T8_O_COL(NX) ((NX) * 128)
 #define T8_PITCH (HD + 4)                  // a row of sums that slices exchange, in floats
 #define LOG2E_F 1.4426950408889634f
 #define T8_ERR_WAIT 9
@@ -133,30 +133,33 @@ kv8_widen_kernel(const uint8_t* __restrict__ cache, size_t page_bytes, const Att
     }
 }
 
-struct T8Smem {
-    static constexpr int kQ = 0;                                  // tile a, tile b
-    static constexpr int kK = kQ + 2 * Q_BYTES;
-    static constexpr int kV = kK + T8_STAGES * KV_BYTES;
-    static constexpr int kBars = kV + T8_STAGES * KV_BYTES;
+template <int NX> struct T8Smem {
+    static constexpr int kQ = 0;
+    static constexpr int kK = kQ + NX * Q_BYTES;
+    static constexpr int kV = kK + T8_STAGES(NX) * KV_BYTES;
+    static constexpr int kBars = kV + T8_STAGES(NX) * KV_BYTES;
     static constexpr int kTotal = kBars + 256 + 1024;             // + alignment slack
-    // slices: [row of both tiles][T8_PITCH], then [row][maximum, sum], over Q, K and V when all is done
+    // slices: [row of the tiles][T8_PITCH], then [row][maximum, sum], over Q, K and V when all is done
     static constexpr int kSums = 0;
-    static constexpr int kStats = 2 * BQ * T8_PITCH * 4;
+    static constexpr int kStats = NX * BQ * T8_PITCH * 4;
+    static_assert(kStats + NX * BQ * 8 <= kBars, "the slices' sums lie over the tiles");
 };
-static_assert(T8Smem::kStats + 2 * BQ * 8 <= T8Smem::kBars, "the slices' sums lie over the tiles");
 
-template <bool SPLIT>
-__global__ void __launch_bounds__(T8_THREADS, 1)
+template <bool SPLIT, int NX>
+__global__ void __launch_bounds__(T8_THREADS(NX), NX == 1 ? 2 : 1)
 attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv,
                              const AttnT8Params p) {
+    using Smem = T8Smem<NX>;
+    constexpr int kStages = T8_STAGES(NX), kLoadWarp = 4 * NX, kMmaWarp = kLoadWarp + 1, kOCol = T8_O_COL(NX);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t* bars = (uint64_t*)(smem + T8Smem::kBars);
+    uint64_t* bars = (uint64_t*)(smem + Smem::kBars);
     uint64_t* q_full = bars + 0;
     uint64_t* k_full = bars + 1;                          // [stage]
     uint64_t* v_full = k_full + 2;                        // [stage]
-    uint64_t* kv_free = v_full + 2;                       // [key tile & 1]: V of that tile and K of the next are read
-    uint64_t* s_full = kv_free + 2;                       // [query tile]
+    uint64_t* k_free = v_full + 2;                        // [stage]
+    uint64_t* v_free = k_free + 2;                        // [stage]
+    uint64_t* s_full = v_free + 2;                        // [query tile]
     uint64_t* p_ready = s_full + 2;                       // [query tile]
     uint64_t* o_full = p_ready + 2;                       // [query tile]: the last product into O is done
     uint32_t* tmem_slot = (uint32_t*)(o_full + 2);
@@ -165,25 +168,15 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     volatile int* s_tile = (volatile int*)(tmem_slot + 3);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per_cta = 2 * p.tokens_per_tile;            // tokens of one CTA
+    const int per_cta = NX * p.tokens_per_tile;           // tokens of one CTA
 
     if (threadIdx.x == 0) {
-        // late portions of a sequence have the most keys to walk: hand them out first
-        // (the KV head is the fast index of the grid: all heads of the longest portions start first)
-        int t = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)p.nkv), found = -1;
-        for (int s = 0; s < p.nseq; ++s) {
-            const int n = p.seq_start[s + 1] - p.seq_start[s];
-            const int nt = (n + per_cta - 1) / per_cta;
-            if (t < nt) { found = s; break; }
-            t -= nt;
-        }
-        *s_seq = *(volatile int*)&g_t8_status != 0 ? -1 : found;       // (after an earlier failure: nothing, but the barriers)
-        *s_tile = t;
         tc::mbar_init(q_full, 1);
         for (int x = 0; x < 2; ++x) {
             tc::mbar_init(&k_full[x], 1);
             tc::mbar_init(&v_full[x], 1);
-            tc::mbar_init(&kv_free[x], 1);
+            tc::mbar_init(&k_free[x], 1);
+            tc::mbar_init(&v_free[x], 1);
             tc::mbar_init(&s_full[x], 1);
             tc::mbar_init(&p_ready[x], 4);                // one arrival per warp of the tile's group
             tc::mbar_init(&o_full[x], 1);
@@ -194,10 +187,36 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         tc::prefetch_tensormap(&tmap_kv);
     }
     // the second query tile starts as zeros: it may not exist
-    for (int i = threadIdx.x; i < Q_BYTES / 16; i += T8_THREADS)
-        reinterpret_cast<uint4*>(smem + T8Smem::kQ + Q_BYTES)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; NX == 2 && i < Q_BYTES / 16; i += T8_THREADS(NX))
+        reinterpret_cast<uint4*>(smem + Smem::kQ + Q_BYTES)[i] = make_uint4(0, 0, 0, 0);
     tc::fence_proxy_async();
-    if (warp == T8_MMA_WARP) tc::tmem_alloc(tmem_slot, T8_TMEM_COLS);
+    if (warp == kMmaWarp) tc::tmem_alloc(tmem_slot, T8_TMEM_COLS(NX));
+    ap_pdl_wait();
+    if (warp == 0) {
+        // late portions of a sequence have the most keys to walk: hand them out first
+        // (the KV head is the fast index of the grid: all heads of the longest portions start first)
+        int t = (int)((gridDim.x - 1 - blockIdx.x) / (unsigned)p.nkv), found = -1;
+        for (int s0 = 0; s0 < p.nseq && found < 0; s0 += 32) {         // 32 sequences' CTAs at once
+            const int s = s0 + lane;
+            int n = s < p.nseq ? (p.seq_start[s + 1] - p.seq_start[s] + per_cta - 1) / per_cta : 0, upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, upto > t);
+            if (past) {
+                found = s0 + __ffs(past) - 1;
+                t -= __shfl_sync(0xffffffffu, upto - n, __ffs(past) - 1);
+            } else {
+                t -= __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        if (lane == 0) {
+            *s_seq = *(volatile int*)&g_t8_status != 0 ? -1 : found;   // (after an earlier failure: nothing, but the barriers)
+            *s_tile = t;
+        }
+    }
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -214,8 +233,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         kvh = (int)(blockIdx.x % (unsigned)p.nkv);
         head0 = kvh * G;
     }
-    const bool has_b = ntok > p.tokens_per_tile;          // the second query tile holds rows
-    ap_pdl_wait();
+    const bool has_b = NX == 2 && ntok > p.tokens_per_tile;          // the second query tile holds rows
     if (active) {
         t8_span(p.positions, row0, ntok, p.window, p.max_blocks * p.P - 1, kmin, kmax);
     }
@@ -237,24 +255,23 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     };
 
     // Registers move from the warps that only issue copies and products to the softmax warps, which hold a row of 128 scores each (the
-    // unit of such a move is four warps): 2 x 224 + 56 = 504 to a thread of each, what the launch holds.
-    if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == T8_LOAD_WARP) {
+    // unit of such a move is four warps): 2 x 224 + 56 = 504 to a thread of each, or 192 + 64 = 256, what the launch holds.
+    if (warp >= kLoadWarp) {
+    if (NX == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == kLoadWarp) {
         if (active && ntiles > 0) {
             if (lane == 0) {
                 tc::mbar_expect_tx(q_full, (uint32_t)((has_b ? 2 : 1) * Q_BYTES));
                 for (int x = 0; x < (has_b ? 2 : 1); ++x)
                     for (int h = 0; h < NHALF; ++h)
-                        tc::tma_load_3d(smem + T8Smem::kQ + x * Q_BYTES + h * SUB_BYTES, &tmap_q, h * 64, head0,
+                        tc::tma_load_3d(smem + Smem::kQ + x * Q_BYTES + h * SUB_BYTES, &tmap_q, h * 64, head0,
                                         row0 + x * p.tokens_per_tile, q_full);
                 const int k_row = (seq * 2 * p.nkv + kvh) * p.cap + t_lo * BKV, v_row = k_row + p.nkv * p.cap;
-                // `after`: the key tile whose turn in the MMA warp frees the stage (kv_free is given one arrival before the first
-                // turn, "tile -1", and one at the end of every turn): K of tile j - 2 was read in turn j - 3, V of it in turn j - 2
-                auto load = [&](int it, int row, uint64_t* full, int after, int base) -> bool {
-                    const int s = it % T8_STAGES;
+                auto load = [&](int it, int row, uint64_t* full, uint64_t* free, int base) -> bool {
+                    const int s = it % kStages;
                     if (*abort_flag) return false;
-                    if (it >= T8_STAGES && !tc::mbar_wait(&kv_free[after & 1], (uint32_t)(((after + (after & 1)) >> 1) & 1))) {
+                    if (!tc::mbar_wait(&free[s], (uint32_t)((it / kStages) & 1) ^ 1)) {
                         *abort_flag = 1;
                         atomicExch(&g_t8_status, T8_ERR_WAIT);
                         return false;
@@ -265,25 +282,26 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                     return true;
                 };
                 // K runs one tile ahead of V
-                bool fine = load(0, k_row, k_full, 0, T8Smem::kK);
+                bool fine = load(0, k_row, k_full, k_free, Smem::kK);
                 for (int it = 0; it < ntiles && fine; ++it) {
-                    if (it + 1 < ntiles) fine = load(it + 1, k_row, k_full, it - 2, T8Smem::kK);
-                    if (fine) fine = load(it, v_row, v_full, it - 2, T8Smem::kV);
+                    if (NX == 1) fine = load(it, v_row, v_full, v_free, Smem::kV);       // (one stage: V of this tile is free first)
+                    if (fine && it + 1 < ntiles) fine = load(it + 1, k_row, k_full, k_free, Smem::kK);
+                    if (NX == 2 && fine) fine = load(it, v_row, v_full, v_free, Smem::kV);
                 }
             }
         }
-    } else if (warp == T8_MMA_WARP) {
+    } else if (warp == kMmaWarp) {
         if (lane == 0 && active && ntiles > 0) {
             constexpr uint32_t idesc_s = tc::instr_desc_bf16_f32(BQ, BKV);
             constexpr uint32_t idesc_o = tc::instr_desc_bf16_f32_b_mn(BQ, HD);
             const int nx = has_b ? 2 : 1;
             // S_x = Q_x K^T of key tile `it`
             auto scores = [&](int it, int x) {
-                const int s = it & 1;
+                const int s = it % kStages;
 #pragma unroll
                 for (int h = 0; h < NHALF; ++h) {
-                    const uint64_t qd = tc::smem_desc_k_major_sw128(smem + T8Smem::kQ + x * Q_BYTES + h * SUB_BYTES);
-                    const uint64_t kd = tc::smem_desc_k_major_sw128(smem + T8Smem::kK + s * KV_BYTES + h * SUB_BYTES);
+                    const uint64_t qd = tc::smem_desc_k_major_sw128(smem + Smem::kQ + x * Q_BYTES + h * SUB_BYTES);
+                    const uint64_t kd = tc::smem_desc_k_major_sw128(smem + Smem::kK + s * KV_BYTES + h * SUB_BYTES);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         tc::mma_bf16(tmem_base + (uint32_t)(x * BKV), qd + 2 * k, kd + 2 * k, idesc_s, (h > 0 || k > 0) ? 1u : 0u);
@@ -295,15 +313,15 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             if (ok) {
                 tc::fence_after_sync();
                 for (int x = 0; x < nx; ++x) scores(0, x);
-                tc::mma_commit(&kv_free[1]);              // "tile -1": K of tile 0 is read
+                tc::mma_commit(&k_free[0]);
             }
             for (int it = 0; it < ntiles && ok; ++it) {
-                const int sv = it & 1;
+                const int sv = it % kStages, sk = (it + 1) % kStages;
                 const bool more = it + 1 < ntiles;
-                ok = tc::mbar_wait(&v_full[sv], (uint32_t)((it >> 1) & 1)) &&
-                     (!more || tc::mbar_wait(&k_full[(it + 1) & 1], (uint32_t)(((it + 1) >> 1) & 1)));
+                ok = tc::mbar_wait(&v_full[sv], (uint32_t)((it / kStages) & 1)) &&
+                     (!more || tc::mbar_wait(&k_full[sk], (uint32_t)(((it + 1) / kStages) & 1)));
                 if (!ok || *abort_flag) break;
-                const uint64_t vd = tc::smem_desc_mn_major_sw128(smem + T8Smem::kV + sv * KV_BYTES, SUB_BYTES);
+                const uint64_t vd = tc::smem_desc_mn_major_sw128(smem + Smem::kV + sv * KV_BYTES, SUB_BYTES);
                 for (int x = 0; x < nx && ok; ++x) {
                     // O_x += P_x V as soon as the tile's group has written P_x (and scaled O_x down where a row's reference
                     // maximum moved); then S_x of the next key tile, which the group turns to while the other tile's products run
@@ -313,13 +331,17 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                     const uint32_t pt = tmem_base + (uint32_t)(x * BKV);      // P_x lies over S_x
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks)
-                        tc::mma_bf16_a_tmem(tmem_base + (uint32_t)(T8_O_COL + x * HD), pt + (uint32_t)(ks * 8),
+                        tc::mma_bf16_a_tmem(tmem_base + (uint32_t)(kOCol + x * HD), pt + (uint32_t)(ks * 8),
                                             vd + (uint64_t)(ks * (16 * 128 / 16)), idesc_o, (it > 0 || ks > 0) ? 1u : 0u);
                     if (!more) tc::mma_commit(&o_full[x]);
+                    if (NX == 1) tc::mma_commit(&v_free[sv]);
                     if (more) scores(it + 1, x);
                 }
                 if (!ok) break;
-                tc::mma_commit(&kv_free[it & 1]);
+                if (more) {
+                    if (NX == 2) tc::mma_commit(&v_free[sv]);
+                    tc::mma_commit(&k_free[sk]);
+                }
             }
             if (!ok && !*abort_flag) {
                 *abort_flag = 1;
@@ -328,7 +350,8 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         }
     }
     } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    if (NX == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     if (active && (warp < 4 || has_b)) {
         // ---- softmax: warps 0..3 own query tile a, warps 4..7 tile b; one row per thread ----
         const int x = warp >> 2;
@@ -338,7 +361,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         const bool rvalid = tok < ntok;
         const uint32_t lane_base = tmem_base + ((uint32_t)(qtr * 32) << 16);
         const uint32_t s_cols = lane_base + (uint32_t)(x * BKV);
-        const uint32_t o_cols = lane_base + (uint32_t)(T8_O_COL + x * HD);
+        const uint32_t o_cols = lane_base + (uint32_t)(kOCol + x * HD);
         const int qpos = p.positions[row0 + (rvalid ? tok : 0)];
         float mref = -INFINITY, l = 0.f;               // the row's reference maximum (log2 units) and sum
         bool ok = true;                                // the same in all lanes of a warp
@@ -448,7 +471,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             // (both query tiles' products are done when this one's are only where there is no other: wait for it before its operands are
             // written over)
             if (has_b && ntiles > 0 && !__all_sync(0xffffffffu, tc::mbar_wait(&o_full[x ^ 1], 0))) ok = false;
-            float* sums = reinterpret_cast<float*>(smem + T8Smem::kSums) + (size_t)(x * BQ + r) * T8_PITCH;
+            float* sums = reinterpret_cast<float*>(smem + Smem::kSums) + (size_t)(x * BQ + r) * T8_PITCH;
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t w[32];
@@ -463,7 +486,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                 for (int d = 0; d < 32; d += 4)
                     *reinterpret_cast<uint4*>(sums + c + d) = make_uint4(w[d], w[d + 1], w[d + 2], w[d + 3]);
             }
-            *reinterpret_cast<float2*>(smem + T8Smem::kStats + (x * BQ + r) * 8) = make_float2(mref, l);
+            *reinterpret_cast<float2*>(smem + Smem::kStats + (x * BQ + r) * 8) = make_float2(mref, l);
         } else {
             const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;     // (a sum that is not a number stays one)
             bf16* dst = p.out + ((size_t)(row0 + (rvalid ? tok : 0)) * p.nh + head0 + hq) * HD;
@@ -493,45 +516,62 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     }
     }
     if (SPLIT) {
-        // Rows' sums of all slices, added up in the slices' order: row i of the CTAs' rows by CTA i % nsplit, a warp to a row
+        // Rows' sums of all slices, added up in the slices' order: row i of the CTAs' rows by CTA i % nsplit, four numbers to a thread
         tc::cluster_sync();
-        const int rows = ntok * G, ns = p.nsplit;
-        for (int i = (int)blockIdx.y + ns * warp; i < rows; i += ns * (T8_THREADS / 32)) {
-            const int tok = i / G, hq = i - tok * G;
-            const uint32_t stats = tc::smem_addr(smem + T8Smem::kStats + i * 8);       // (tile b's rows lie behind tile a's)
-            const uint32_t sums = tc::smem_addr(smem + T8Smem::kSums) + (uint32_t)(i * T8_PITCH + lane * (HD / 32)) * 4u;
-            float M = -INFINITY, L = 0.f, O[HD / 32];
+        const int ns = p.nsplit, rank = (int)blockIdx.y, mine = (ntok * G - rank + ns - 1) / ns;
+        constexpr int kAtOnce = 4;
+        for (int k0 = threadIdx.x; warp < kLoadWarp && k0 < mine * (HD / 4); k0 += kAtOnce * NX * 128) {
+            uint32_t stats[kAtOnce], sums[kAtOnce];
+            float M[kAtOnce], L[kAtOnce];
+            float4 O[kAtOnce];
 #pragma unroll
-            for (int e = 0; e < HD / 32; ++e) O[e] = 0.f;
-            for (int z = 0; z < ns; ++z) {
-                const uint32_t st = tc::map_to_rank(stats, (uint32_t)z), su = tc::map_to_rank(sums, (uint32_t)z);
-                float m, l, o[HD / 32];
-                asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m), "=f"(l) : "r"(st));
-                if constexpr (HD == 128)
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o[0]), "=f"(o[1]), "=f"(o[2]), "=f"(o[3]) : "r"(su));
-                else
-                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(o[0]), "=f"(o[1]) : "r"(su));
-                const float m_new = fmaxf(M, m), use = m_new == -INFINITY ? 0.f : m_new;
-                const float f = t8_exp2(M - use), fz = t8_exp2(m - use);
-                M = m_new;
-                L = L * f + l * fz;
-#pragma unroll
-                for (int e = 0; e < HD / 32; ++e) O[e] = O[e] * f + o[e] * fz;
+            for (int e = 0; e < kAtOnce; ++e) {
+                const int k = min(k0 + e * NX * 128, mine * (HD / 4) - 1), i = rank + k / (HD / 4) * ns;
+                stats[e] = tc::smem_addr(smem + Smem::kStats + i * 8);              // (tile b's rows lie behind tile a's)
+                sums[e] = tc::smem_addr(smem + Smem::kSums) + (uint32_t)(i * T8_PITCH + k % (HD / 4) * 4) * 4u;
+                M[e] = -INFINITY;
+                L[e] = 0.f;
+                O[e] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            bf16* dst = p.out + ((size_t)(row0 + tok) * p.nh + head0 + hq) * HD + lane * (HD / 32);
+            for (int z = 0; z < ns; ++z) {
+                float m[kAtOnce], l[kAtOnce];
+                float4 o[kAtOnce];
 #pragma unroll
-            for (int e = 0; e < HD / 32; e += 2)
-                *reinterpret_cast<__nv_bfloat162*>(dst + e) = __floats2bfloat162_rn(O[e] * inv, O[e + 1] * inv);
+                for (int e = 0; e < kAtOnce; ++e) {
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[e]), "=f"(l[e]) : "r"(tc::map_to_rank(stats[e], (uint32_t)z)));
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(o[e].x), "=f"(o[e].y), "=f"(o[e].z), "=f"(o[e].w) : "r"(tc::map_to_rank(sums[e], (uint32_t)z)));
+                }
+#pragma unroll
+                for (int e = 0; e < kAtOnce; ++e) {
+                    const float m_new = fmaxf(M[e], m[e]), use = m_new == -INFINITY ? 0.f : m_new;
+                    const float f = t8_exp2(M[e] - use), fz = t8_exp2(m[e] - use);
+                    M[e] = m_new;
+                    L[e] = L[e] * f + l[e] * fz;
+                    O[e].x = O[e].x * f + o[e].x * fz; O[e].y = O[e].y * f + o[e].y * fz;
+                    O[e].z = O[e].z * f + o[e].z * fz; O[e].w = O[e].w * f + o[e].w * fz;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
+                const int k = k0 + e * NX * 128, i = rank + k / (HD / 4) * ns, tok = i / G, hq = i - tok * G;
+                if (k >= mine * (HD / 4)) continue;
+                const float inv = L[e] == 0.f ? 0.f : 1.f / L[e];
+                uint2 v;
+                __nv_bfloat162* v2 = reinterpret_cast<__nv_bfloat162*>(&v);
+                v2[0] = __floats2bfloat162_rn(O[e].x * inv, O[e].y * inv);
+                v2[1] = __floats2bfloat162_rn(O[e].z * inv, O[e].w * inv);
+                *reinterpret_cast<uint2*>(p.out + ((size_t)(row0 + tok) * p.nh + head0 + hq) * HD + k % (HD / 4) * 4) = v;
+            }
         }
         tc::cluster_sync();                                // nobody leaves while its sums may be read
     }
     tc::fence_before_sync();
     __syncthreads();
     ap_pdl_trigger();
-    if (warp == T8_MMA_WARP) {
+    if (warp == kMmaWarp) {
         __syncwarp();
-        tc::tmem_dealloc(tmem_base, T8_TMEM_COLS);
+        tc::tmem_dealloc(tmem_base, T8_TMEM_COLS(NX));
     }
 }
 
@@ -560,19 +600,19 @@ AP_EXPORT int ap_attention_kv8_tcgen05_takes(int nh, int nkv, int hd, int P) {
     return t8_encode_fn() != nullptr;
 }
 
-// tokens of one sequence that one CTA takes (two query tiles)
-AP_EXPORT int ap_attention_kv8_tcgen05_tokens(int nh, int nkv) { return 2 * (128 / (nh / nkv)); }
+// tokens of one sequence in a query tile
+AP_EXPORT int ap_attention_kv8_tcgen05_tokens(int nh, int nkv) { return 128 / (nh / nkv); }
 
 // Bytes of scratch for `nseq` sequences with block tables of `max_blocks` pages
 AP_EXPORT long long ap_attention_kv8_tcgen05_scratch(int nseq, int max_blocks, int P, int nkv) {
     return 2LL * nseq * 2 * nkv * (((long long)max_blocks * P + BKV - 1) / BKV * BKV) * HD;
 }
 
-// q: [T][nh][HD]; total_ctas: the sum over the sequences of ceil(rows / tokens of a CTA); nsplit: 1, 2, 4 or 8 key slices; scale > 0;
+// q: [T][nh][HD]; query_tiles: 1 or 2 to a CTA; total_ctas: the sum over the sequences of ceil(rows / tokens of a CTA); nsplit: 1, 2, 4 or 8 key slices; scale > 0;
 // scratch: ap_attention_kv8_tcgen05_scratch bytes of any contents, 16-byte aligned, of no call that runs at the same time.
 AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cache, long long num_pages, long long page_bytes,
                                        const int* block_table, int max_blocks, const int* seq_start, const int* positions, int nseq, int T,
-                                       int nh, int nkv, int hd, int P, float scale, int window, int total_ctas, int nsplit, void* scratch,
+                                       int nh, int nkv, int hd, int P, float scale, int window, int query_tiles, int total_ctas, int nsplit, void* scratch,
                                        long long scratch_bytes, cudaStream_t stream) {
     AP_REQUIRE(ap_attention_kv8_tcgen05_takes(nh, nkv, hd, P), "attention_kv8 (tcgen05): shape not supported: heads=%d kv_heads=%d "
                "head_dim=%d page=%d", nh, nkv, hd, P);
@@ -584,8 +624,9 @@ AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cac
     AP_REQUIRE(dense_rows < (1LL << 31) - 256, "attention_kv8 (tcgen05): %lld rows of keys and values are too many", dense_rows);
     AP_REQUIRE(scratch && scratch_bytes >= ap_attention_kv8_tcgen05_scratch(nseq, max_blocks, P, nkv), "attention_kv8 (tcgen05): %lld bytes of "
                "scratch are too few", scratch_bytes);
+    AP_REQUIRE(query_tiles == 1 || query_tiles == 2, "attention_kv8 (tcgen05): %d query tiles", query_tiles);
     AP_REQUIRE(scale > 0.f, "attention_kv8 (tcgen05): the scale must be positive");
-    AP_REQUIRE(nsplit == 1 || nsplit == 2 || nsplit == 4 || nsplit == 8, "attention_kv8: bad number of key slices %d", nsplit);
+    AP_REQUIRE(nsplit >= 1 && nsplit <= 8 && (nsplit & (nsplit - 1)) == 0, "attention_kv8: bad number of key slices %d", nsplit);
     AP_REQUIRE(nseq <= 65535 && 2 * nkv <= 65535, "attention_kv8 (tcgen05): %d sequences of %d KV heads exceed the grid", nseq, nkv);
     const int G = nh / nkv;
     CUtensorMap mq, mkv;
@@ -613,10 +654,14 @@ AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cac
     int dev = 0;
     AP_REQUIRE(cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64, "attention_kv8: cannot tell the current device");
     if (!configured[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(attention_kv8_tcgen05_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, T8Smem::kTotal);
+        cudaError_t e = cudaFuncSetAttribute(attention_kv8_tcgen05_kernel<false, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, T8Smem<1>::kTotal);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attention_kv8_tcgen05_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, T8Smem::kTotal);
-        AP_REQUIRE(e == cudaSuccess, "attention_kv8 (tcgen05): cannot reserve %d bytes of shared memory: %s", T8Smem::kTotal,
+            e = cudaFuncSetAttribute(attention_kv8_tcgen05_kernel<true, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, T8Smem<1>::kTotal);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(attention_kv8_tcgen05_kernel<false, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, T8Smem<2>::kTotal);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(attention_kv8_tcgen05_kernel<true, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, T8Smem<2>::kTotal);
+        AP_REQUIRE(e == cudaSuccess, "attention_kv8 (tcgen05): cannot reserve %d bytes of shared memory: %s", T8Smem<2>::kTotal,
                    cudaGetErrorString(e));
         configured[dev] = true;
     }
@@ -630,8 +675,8 @@ AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cac
                                                      (const uint8_t*)cache, (size_t)page_bytes, p, (bf16*)scratch));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(total_ctas * nkv), nsplit);
-    cfg.blockDim = dim3(T8_THREADS);
-    cfg.dynamicSmemBytes = T8Smem::kTotal;
+    cfg.blockDim = dim3(T8_THREADS(query_tiles));
+    cfg.dynamicSmemBytes = query_tiles == 1 ? T8Smem<1>::kTotal : T8Smem<2>::kTotal;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -642,8 +687,11 @@ AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cac
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = nsplit > 1 ? 2 : 1;
-    AP_CHECK_PDL_LAUNCH("attention_kv8_tcgen05", nsplit > 1 ? cudaLaunchKernelEx(&cfg, attention_kv8_tcgen05_kernel<true>, mq, mkv, p)
-                                                            : cudaLaunchKernelEx(&cfg, attention_kv8_tcgen05_kernel<false>, mq, mkv, p));
+    AP_CHECK_PDL_LAUNCH("attention_kv8_tcgen05",
+                        query_tiles == 1 ? (nsplit > 1 ? cudaLaunchKernelEx(&cfg, attention_kv8_tcgen05_kernel<true, 1>, mq, mkv, p)
+                                                       : cudaLaunchKernelEx(&cfg, attention_kv8_tcgen05_kernel<false, 1>, mq, mkv, p))
+                                         : (nsplit > 1 ? cudaLaunchKernelEx(&cfg, attention_kv8_tcgen05_kernel<true, 2>, mq, mkv, p)
+                                                       : cudaLaunchKernelEx(&cfg, attention_kv8_tcgen05_kernel<false, 2>, mq, mkv, p)));
     return AP_OK;
 }
 

@@ -178,19 +178,31 @@ def _rows(q, out, cache_layer, block_table, token_seq, positions, first, rows, n
 
 @functools.lru_cache(maxsize=None)
 def _portions_taken(num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> int:
-    """Tokens of a sequence to a CTA of the kernel for portions (0: it does not take the shape)."""
+    """Tokens of a sequence in a query tile of the kernel for portions (0: it does not take the shape)."""
     lib = library.attention(head_dim)
     if not lib.ap_attention_kv8_tcgen05_takes(num_heads, num_kv_heads, head_dim, page_size):
         return 0
     return int(lib.ap_attention_kv8_tcgen05_tokens(num_heads, num_kv_heads))
 
 
-def plan_portions(ctas: int, tiles: int, sms: int) -> int:
-    """Key slices of the kernel for portions: ``ctas`` CTAs before slicing, rows that see up to ``tiles`` tiles of 128 keys."""
+def plan_portions(query_lens: Sequence[int], per_tile: int, num_kv_heads: int, keys: int, sms: int):
+    """(query tiles to a CTA, CTAs to a KV head, key slices) of the kernel for portions: query tiles of ``per_tile`` tokens, rows that see
+    some ``keys`` keys on average.
+
+    Measured (one B200, 32 heads on 8 KV heads of 128, us).  Two query tiles share every key tile, and a CTA with only one of them
+    filled is no slower alone on its SM (2048 rows behind nothing: 58, one tile 68; 17 behind 8191: 37.7, one tile 38.4); but two CTAs of
+    one tile fit an SM, so one tile is taken where CTAs outnumber the SMs and a tenth of the second tiles would lie empty (32 sequences of
+    2 rows and 2000 keys: 125, two tiles 138; twelve prompts of 21 to 515 on heads of 64: 32.6, two tiles 35.8).  The keys are cut
+    while CTAs are fewer than SMs and a slice keeps some two tiles of 128 keys (512 rows behind 4096 keys: 61 in two, 90 whole; behind
+    nothing: 27 in two, 24 whole; 17 behind 1000: 20.5 in four, 21.6 in eight; 12 sequences of 32 rows and 1000 keys: 60 in two, 44 whole)."""
+    single = sum(-(-n // per_tile) for n in query_lens)
+    ctas = sum(-(-n // (2 * per_tile)) for n in query_lens)
+    if ctas * num_kv_heads > sms and 10 * single <= 19 * ctas:
+        return 1, single, 1
     slices = 1
-    while slices < 8 and ctas * slices * 2 <= sms and tiles >= 4 * slices:
+    while slices < 8 and ctas * num_kv_heads * slices * 2 <= sms and keys >= 480 * slices:
         slices *= 2
-    return slices
+    return 2, ctas, slices
 
 
 # bytes of scratch for widened keys and values up to which sequences go together
@@ -198,23 +210,23 @@ WIDE_SCRATCH = 1 << 30
 
 
 def _portions(q, out, cache_layer, block_table, seq_start, positions, first_seq, query_lens, T, num_heads, num_kv_heads, head_dim,
-              page_size, scale, window, per_cta, scratch, device) -> None:
-    """The sequences from ``first_seq`` on, by their ``query_lens``; their rows follow those of the sequences before."""
+              page_size, scale, window, per_tile, longest, scratch, device) -> None:
+    """The sequences from ``first_seq`` on, by their ``query_lens``, of up to ``longest`` keys; their rows follow those of the sequences
+    before."""
     width, lib = block_table.shape[1], library.attention(head_dim)
     one = lib.ap_attention_kv8_tcgen05_scratch(1, width, page_size, num_kv_heads)
     step = max(1, min(len(query_lens), WIDE_SCRATCH // one))
     buf = scratch("attn.kv8_wide", (step * one // 2,), torch.bfloat16) if scratch is not None else \
         torch.empty(step * one // 2, dtype=torch.bfloat16, device=q.device)
-    keys = min(width * page_size, window + per_cta) if window else width * page_size
+    longest = min(longest, window + max(query_lens)) if window else longest
     for at in range(0, len(query_lens), step):
-        n = min(step, len(query_lens) - at)
-        ctas = sum(-(-rows // per_cta) for rows in query_lens[at:at + n])
+        lens = query_lens[at:at + step]
+        query_tiles, ctas, slices = plan_portions(lens, per_tile, num_kv_heads, longest - max(lens) // 2, _sms(device))
         if ctas:
             call(lib, "ap_attention_kv8_tcgen05", q.data_ptr(), out.data_ptr(), cache_layer.data_ptr(), cache_layer.shape[0],
                  cache_layer.shape[1], block_table.data_ptr() + 4 * (first_seq + at) * width, width,
-                 seq_start.data_ptr() + 4 * (first_seq + at), positions.data_ptr(), n, T, num_heads, num_kv_heads, head_dim, page_size,
-                 float(scale), int(window), ctas, plan_portions(ctas * num_kv_heads, -(-keys // 128), _sms(device)), buf.data_ptr(),
-                 step * one, stream_handle())
+                 seq_start.data_ptr() + 4 * (first_seq + at), positions.data_ptr(), len(lens), T, num_heads, num_kv_heads, head_dim,
+                 page_size, float(scale), int(window), query_tiles, ctas, slices, buf.data_ptr(), step * one, stream_handle())
 
 
 def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor, block_table: torch.Tensor,
@@ -249,10 +261,11 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
             while ones < len(query_lens) and query_lens[ones] == 1:
                 ones += 1
             if ones < len(query_lens):
-                per_cta = _portions_taken(num_heads, num_kv_heads, head_dim, page_size) if scale > 0 else 0
-                if per_cta:
+                per_tile = _portions_taken(num_heads, num_kv_heads, head_dim, page_size) if scale > 0 else 0
+                if per_tile:
                     _portions(q, out, cache_layer, block_table, seq_start, positions, ones, query_lens[ones:], T, num_heads,
-                              num_kv_heads, head_dim, page_size, scale, window, per_cta, scratch, device)
+                              num_kv_heads, head_dim, page_size, scale, window, per_tile, max_context if max_context and not ones else widest,
+                              scratch, device)
                     rows = ones
         if rows:
             longest = max_context if max_context and rows == ones else widest

@@ -276,13 +276,14 @@ def test_any_cut_of_the_work(ops, ctas, cluster, nh, nkv, hd, P, monkeypatch):
         check(run(ops, c, 0.09), c, 0.09)
 
 
-@pytest.mark.parametrize("slices", [1, 2, 4, 8])
+@pytest.mark.parametrize("query_tiles,slices", [(1, 1), (1, 2), (1, 4), (1, 8), (2, 1), (2, 2), (2, 4), (2, 8)])
 @pytest.mark.parametrize("nh,nkv,hd,P", [(8, 2, 128, 16), (16, 1, 128, 64), (32, 2, 64, 8), (4, 4, 64, 128), (128, 1, 64, 256), (8, 8, 128, 32)])
 @pytest.mark.parametrize("window", [0, 100])
-def test_portions_on_tensor_cores(ops, slices, nh, nkv, hd, P, window, monkeypatch):
+def test_portions_on_tensor_cores(ops, query_tiles, slices, nh, nkv, hd, P, window, monkeypatch):
     """Portions of two rows to several CTAs' worth, key slices that hold many tiles, one or none, one-row sequences among them."""
     from allpaca_b200.ops import kv8
-    monkeypatch.setattr(kv8, "plan_portions", lambda *a: slices)
+    monkeypatch.setattr(kv8, "plan_portions", lambda lens, per_tile, *a: (
+        query_tiles, sum(-(-n // (query_tiles * per_tile)) for n in lens), slices))
     monkeypatch.setattr(kv8, "WIDE_SCRATCH", (1 << 30) if slices < 4 else 1)          # all sequences together, or one by one
     for seqs in ([(1500, 2), (700, 70), (129, 129), (1, 1), (64, 1), (2, 2), (3000, 300)], [(130, 130)], [(257, 2)]):
         c = plain.case(seqs, nh, nkv, hd, P, torch.bfloat16, seed=slices + hd)
