@@ -10,131 +10,115 @@
 
 #define KV8_THREADS 256
 
-// sums of S slices of eight neighbouring numbers, in the slices' order
-template <typename TI> __device__ __forceinline__ void kv8_load8(float (&x)[8], const TI* p, int S, size_t stride);
-template <> __device__ __forceinline__ void kv8_load8<float>(float (&x)[8], const float* p, int S, size_t stride) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+// sums of S slices of four neighbouring numbers, in the slices' order
+template <typename TI> __device__ __forceinline__ float4 kv8_load4(const TI* p, int S, size_t stride);
+template <> __device__ __forceinline__ float4 kv8_load4<float>(const float* p, int S, size_t stride) {
+    float4 x = *reinterpret_cast<const float4*>(p);
     for (int s = 1; s < S; ++s) {
         p += stride;
-        const float4 c = *reinterpret_cast<const float4*>(p), d = *reinterpret_cast<const float4*>(p + 4);
-        x[0] += c.x; x[1] += c.y; x[2] += c.z; x[3] += c.w; x[4] += d.x; x[5] += d.y; x[6] += d.z; x[7] += d.w;
+        const float4 c = *reinterpret_cast<const float4*>(p);
+        x.x += c.x; x.y += c.y; x.z += c.z; x.w += c.w;
     }
+    return x;
 }
-template <> __device__ __forceinline__ void kv8_load8<bf16>(float (&x)[8], const bf16* p, int, size_t) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+template <> __device__ __forceinline__ float4 kv8_load4<bf16>(const bf16* p, int, size_t) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xffff0000u));
 }
-__device__ __forceinline__ void kv8_store8(float* p, const float* x) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ __forceinline__ void kv8_store8(bf16* p, const float* x) {
-    uint4 u;
+__device__ __forceinline__ void kv8_store4(float* p, const float4 x) { *reinterpret_cast<float4*>(p) = x; }
+__device__ __forceinline__ void kv8_store4(bf16* p, const float4 x) {
+    uint2 u;
     __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+    h[0] = __floats2bfloat162_rn(x.x, x.y);
+    h[1] = __floats2bfloat162_rn(x.z, x.w);
+    *reinterpret_cast<uint2*>(p) = u;
+}
+// the largest magnitude among the finite ones
+__device__ __forceinline__ uint32_t kv8_largest(uint32_t m, const float4 x) {
+    const uint32_t u[4] = {__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu, __float_as_uint(x.z) & 0x7fffffffu,
+                           __float_as_uint(x.w) & 0x7fffffffu};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = u;
+    for (int i = 0; i < 4; ++i) m = max(m, u[i] < 0x7f800000u ? u[i] : 0u);
+    return m;
+}
+// x * f as four numbers of 8 bits (x - x: 0, or NaN where x is not finite)
+__device__ __forceinline__ uint32_t kv8_round4(const float4 x, float f) {
+    return kv8_pack4(fmaf(x.x, f, x.x - x.x), fmaf(x.y, f, x.y - x.y), fmaf(x.z, f, x.z - x.z), fmaf(x.w, f, x.w - x.w));
 }
 
-// LPH lanes side by side take a head of a row (hd / 16 of them work): a lane holds numbers i .. i + 7 and i + hd/2 .. i + hd/2 + 7,
-// i = 8 * lane, which are eight whole pairs of the rotation; the maximum goes round the lanes in registers, so the row is read
+// LPH lanes side by side take a head of a row (hd / 8 of them work): a lane holds numbers i .. i + 3 and i + hd/2 .. i + hd/2 + 3,
+// i = 4 * lane, which are four whole pairs of the rotation; the maximum goes round the lanes in registers, so the row is read
 // and written once.  The products of the rotation are rounded one by one (no fused multiply-add), so that the same inputs give the
 // same bytes as the formula computed step by step.
+//
+// Few rows are bound by their launch and three loads that wait for one another (position, page, store): 1 row of a small model 2.5 us,
+// 64 rows 2.1 in a stream of such launches.  Many rows are bound by the time a warp is alive, from its first load to its last store: 2048
+// rows of 32 + 16 heads of 128 (47 MB, floor 7.3 us) take 14.3 us, 8192 rows 50.2.  Eight numbers to a half and lane, rows of
+// a prompt in turns of CTAs of 128 threads, were 13.3 and 42.6, but 64 rows 3.1; several heads to a thread with all loads ahead
+// were slower everywhere (two 19.4 for 2048 rows, four 29.9), and so was looking the page up ahead of the rotation (16.1).
 template <typename TI, typename TO, int LPH>
-__global__ void __launch_bounds__(KV8_THREADS)
+__global__ void __launch_bounds__(KV8_THREADS, 6)
 rope_kv8_store_kernel(const TI* __restrict__ in, int S, size_t in_stride, TO* __restrict__ q_out, uint8_t* __restrict__ cache,
                       const int* __restrict__ positions, const int* __restrict__ token_seq, const int* __restrict__ block_table,
-                      int max_blocks, int nseq, const float2* __restrict__ cos_sin, int pairing, int nh, int nkv, int hd, int P,
-                      size_t page_bytes, int num_pages, int chunks, int heads) {
-    const int t = blockIdx.x / chunks;
-    const int head = (blockIdx.x - t * chunks) * (KV8_THREADS / LPH) + threadIdx.x / LPH;
-    const int lane = threadIdx.x & (LPH - 1), half = hd >> 1, i = lane * 8;
+                      int max_blocks, int nseq, const float2* __restrict__ cos_sin, int pairing, int T, int nh, int nkv, int hd, int P,
+                      size_t page_bytes, int num_pages) {
+    const int heads = nh + 2 * nkv, lane = threadIdx.x & (LPH - 1), half = hd >> 1, i = lane * 4;
+    const unsigned id = blockIdx.x * (KV8_THREADS / LPH) + threadIdx.x / LPH;      // (fewer than 2^31: the launch checks)
+    const int t = (int)(id / (unsigned)heads), head = (int)(id - (unsigned)t * (unsigned)heads);
     ap_pdl_trigger();
     ap_pdl_wait();
-    const bool works = head < heads && i < half;
-    float a[8], b[8];
+    const bool works = t < T && i < half, turns = head < nh + nkv;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    int at_a = i, at_b = i + half;                            // where the results go
     if (works) {
-        const TI* src = in + ((size_t)t * (nh + 2 * nkv) + head) * hd;
-        const bool pairs_side_by_side = pairing != 0 && head < nh + nkv;
-        const int ia = pairs_side_by_side ? 2 * i : i, ib = pairs_side_by_side ? 2 * i + 8 : i + half;
-        kv8_load8<TI>(a, src + ia, S, in_stride);
-        kv8_load8<TI>(b, src + ib, S, in_stride);
-        if (pairs_side_by_side) {
-            float x[8], y[8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                x[k] = a[2 * k];     y[k] = a[2 * k + 1];
-                x[k + 4] = b[2 * k]; y[k + 4] = b[2 * k + 1];
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) a[k] = x[k], b[k] = y[k];
+        const TI* src = in + (size_t)id * hd;
+        const bool pairs = turns && pairing != 0;
+        a = kv8_load4<TI>(src + (pairs ? 2 * i : i), S, in_stride);
+        b = kv8_load4<TI>(src + (pairs ? 2 * i + 4 : i + half), S, in_stride);
+        if (pairs) {
+            const float4 x = a;
+            a = make_float4(x.x, x.z, b.x, b.z);
+            b = make_float4(x.y, x.w, b.y, b.w);
         }
-        if (cos_sin && head < nh + nkv) {
+        if (cos_sin && turns) {
             const float4* cs = reinterpret_cast<const float4*>(cos_sin + (size_t)t * half + i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float4 c = cs[k];                       // (cos, sin) of pairs 2k and 2k + 1
-                const float a0 = a[2 * k], b0 = b[2 * k], a1 = a[2 * k + 1], b1 = b[2 * k + 1];
-                a[2 * k] = __fsub_rn(__fmul_rn(a0, c.x), __fmul_rn(b0, c.y));
-                b[2 * k] = __fadd_rn(__fmul_rn(a0, c.y), __fmul_rn(b0, c.x));
-                a[2 * k + 1] = __fsub_rn(__fmul_rn(a1, c.z), __fmul_rn(b1, c.w));
-                b[2 * k + 1] = __fadd_rn(__fmul_rn(a1, c.w), __fmul_rn(b1, c.z));
-            }
+            const float4 c = cs[0], d = cs[1], x = a;         // (cos, sin) of two pairs each
+            a = make_float4(__fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(b.x, c.y)), __fsub_rn(__fmul_rn(x.y, c.z), __fmul_rn(b.y, c.w)),
+                            __fsub_rn(__fmul_rn(x.z, d.x), __fmul_rn(b.z, d.y)), __fsub_rn(__fmul_rn(x.w, d.z), __fmul_rn(b.w, d.w)));
+            b = make_float4(__fadd_rn(__fmul_rn(x.x, c.y), __fmul_rn(b.x, c.x)), __fadd_rn(__fmul_rn(x.y, c.w), __fmul_rn(b.y, c.z)),
+                            __fadd_rn(__fmul_rn(x.z, d.y), __fmul_rn(b.z, d.x)), __fadd_rn(__fmul_rn(x.w, d.w), __fmul_rn(b.w, d.z)));
         }
-        if (pairing == 1 && head < nh + nkv) {                // the results are neighbours as well: a: 2i .. 2i + 7, b: 2i + 8 ..
-            float x[8], y[8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                x[2 * k] = a[k];     x[2 * k + 1] = b[k];
-                y[2 * k] = a[k + 4]; y[2 * k + 1] = b[k + 4];
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) a[k] = x[k], b[k] = y[k];
+        if (turns && pairing == 1) {                          // the results are neighbours as well
+            const float4 x = a;
+            a = make_float4(x.x, b.x, x.y, b.y);
+            b = make_float4(x.z, b.z, x.w, b.w);
+            at_a = 2 * i;
+            at_b = 2 * i + 4;
         }
-        const int oa = pairing == 1 && head < nh + nkv ? 2 * i : i;
-        const int ob = pairing == 1 && head < nh + nkv ? 2 * i + 8 : i + half;
         if (head < nh) {
             TO* dst = q_out + ((size_t)t * nh + head) * hd;
-            kv8_store8(dst + oa, a);
-            kv8_store8(dst + ob, b);
+            kv8_store4(dst + at_a, a);
+            kv8_store4(dst + at_b, b);
         }
     }
     // (warp-wide from here on, as the lanes of a head exchange their maxima)
-    uint32_t amax = 0;
-    if (works && head >= nh) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t ua = __float_as_uint(a[k]) & 0x7fffffffu, ub = __float_as_uint(b[k]) & 0x7fffffffu;
-            amax = max(amax, ua < 0x7f800000u ? ua : 0u);
-            amax = max(amax, ub < 0x7f800000u ? ub : 0u);
-        }
-    }
+    const bool kept = works && head >= nh;
+    if (!__any_sync(0xffffffffu, kept)) return;
+    uint32_t amax = kv8_largest(kv8_largest(0u, a), b);
 #pragma unroll
     for (int o = LPH / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (!works || head < nh) return;
+    if (!kept) return;
     const int pos = positions[t], seq = token_seq[t];
     if (pos < 0 || pos / P >= max_blocks || seq < 0 || seq >= nseq) return;
     const int page = block_table[(size_t)seq * max_blocks + pos / P];
     if (page < 0 || page >= num_pages) return;                // a row without a page is not kept
     const int byte = kv8_scale_byte(amax);
     const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);     // 2^-e
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {                             // x - x: 0, or NaN where x is not finite
-        a[k] = fmaf(a[k], inv, a[k] - a[k]);
-        b[k] = fmaf(b[k], inv, b[k] - b[k]);
-    }
-    const int which = head >= nh + nkv ? 1 : 0, kvh = head - nh - which * nkv;
-    const int oa = pairing == 1 && !which ? 2 * i : i, ob = pairing == 1 && !which ? 2 * i + 8 : i + half;
-    const size_t row = (size_t)(which * nkv + kvh) * P + pos % P;
+    const size_t row = (size_t)(head - nh) * P + pos % P;
     uint8_t* base = cache + (size_t)page * page_bytes;
-    *reinterpret_cast<uint2*>(base + row * hd + oa) = make_uint2(kv8_pack4(a[0], a[1], a[2], a[3]), kv8_pack4(a[4], a[5], a[6], a[7]));
-    *reinterpret_cast<uint2*>(base + row * hd + ob) = make_uint2(kv8_pack4(b[0], b[1], b[2], b[3]), kv8_pack4(b[4], b[5], b[6], b[7]));
+    *reinterpret_cast<uint32_t*>(base + row * hd + at_a) = kv8_round4(a, inv);
+    *reinterpret_cast<uint32_t*>(base + row * hd + at_b) = kv8_round4(b, inv);
     if (lane == 0) base[(size_t)2 * nkv * P * hd + row] = (uint8_t)byte;
 }
 
@@ -161,22 +145,22 @@ AP_EXPORT int ap_rope_kv8_store(const void* in, int in_dtype, int S, long long i
                "rope_kv8_store: operands must be 16-byte aligned");
     AP_REQUIRE(in_dtype == AP_F32 || S == 1, "rope_kv8_store: partial sums must be 32-bit");
     if (T == 0) return AP_OK;
-    const int heads = nh + 2 * nkv, lanes = hd / 16;
-    const int lph = lanes <= 1 ? 1 : lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
-    const int per = KV8_THREADS / lph, chunks = (heads + per - 1) / per;
-    AP_REQUIRE((long long)T * chunks < (1LL << 31), "rope_kv8_store: %d rows exceed the grid", T);
-    const dim3 grid((unsigned)((long long)T * chunks));
-#define KV8_STORE(TI, TO, L)                                                                                                     \
-    AP_CHECK_PDL_LAUNCH("rope_kv8_store", ap_launch_pdl(rope_kv8_store_kernel<TI, TO, L>, grid, dim3(KV8_THREADS), 0, stream,     \
+    const int heads = nh + 2 * nkv, lanes = hd / 8;
+    const int lph = lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
+    const int per = KV8_THREADS / lph;
+    AP_REQUIRE((long long)T * heads < (1LL << 31) - per, "rope_kv8_store: %d rows of %d heads exceed the grid", T, heads);
+    const unsigned ctas = (unsigned)(((long long)T * heads + per - 1) / per);
+#define KV8_STORE(TI, TO, L)                                                                                                        \
+    AP_CHECK_PDL_LAUNCH("rope_kv8_store", ap_launch_pdl(rope_kv8_store_kernel<TI, TO, L>, dim3(ctas), dim3(KV8_THREADS), 0, stream,  \
                         (const TI*)in, S, (size_t)in_stride, (TO*)q_out, (uint8_t*)cache, positions, token_seq, block_table, max_blocks, \
-                        nseq, (const float2*)cos_sin, pairing, nh, nkv, hd, P, (size_t)page_bytes, (int)num_pages, chunks, heads))
+                        nseq, (const float2*)cos_sin, pairing, T, nh, nkv, hd, P, (size_t)page_bytes, (int)num_pages))
 #define KV8_STORE_BY_LANES(TI, TO)                  \
     do {                                            \
-        if (lph == 1) KV8_STORE(TI, TO, 1);         \
-        else if (lph == 2) KV8_STORE(TI, TO, 2);    \
+        if (lph == 2) KV8_STORE(TI, TO, 2);         \
         else if (lph == 4) KV8_STORE(TI, TO, 4);    \
         else if (lph == 8) KV8_STORE(TI, TO, 8);    \
-        else KV8_STORE(TI, TO, 16);                 \
+        else if (lph == 16) KV8_STORE(TI, TO, 16);  \
+        else KV8_STORE(TI, TO, 32);                 \
     } while (0)
     if (in_dtype == AP_F32 && act_dtype == AP_F32) KV8_STORE_BY_LANES(float, float);
     else if (in_dtype == AP_F32 && act_dtype == AP_BF16) KV8_STORE_BY_LANES(float, bf16);
@@ -187,44 +171,64 @@ AP_EXPORT int ap_rope_kv8_store(const void* in, int in_dtype, int S, long long i
     return AP_OK;
 }
 
-// Reading back: a thread takes 16 numbers of a row of a head (one 16-byte load, one scale); neighbouring threads write
-// neighbouring runs of the output.
+// Reading back: a CTA takes `tile` rows of one head's keys or values.  Its first threads look up where the rows lie and their scales; then
+// runs = hd / 8 threads side by side take a row, eight numbers (one 8-byte load, two stores) to each, eight rows to a thread
+// with all eight loads under way.
+//
+// Bound by memory: 42,300 rows of 16 sequences, 8 KV heads of 128, to bfloat16 (260 MB, floor 40.4 us at the copy rate) take 44.2 us,
+// 5.9 TB/s, pages scattered.  What counts is loads in flight: 51.3 us with four rows to a thread, 67.4 with two, 46.6 with
+// sixteen; 62.4 with sixteen numbers of one row to a thread and its place looked up by every thread.  CTAs of 256 threads: 45.3.
+#define KV8_READ_THREADS 128
+#define KV8_READ_ROWS 8
 template <typename TO>
-__global__ void __launch_bounds__(KV8_THREADS)
+__global__ void __launch_bounds__(KV8_READ_THREADS)
 kv8_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ positions, const int* __restrict__ token_seq,
                 const int* __restrict__ block_table, int max_blocks, int nseq, TO* __restrict__ k_out, TO* __restrict__ v_out, int T,
                 int nkv, int hd, int P, size_t page_bytes, int num_pages) {
-    const int runs = hd / 16, per_row = 2 * nkv * runs;
+    __shared__ long long at_s[KV8_READ_ROWS * KV8_READ_THREADS / 2];        // where a row's numbers lie (-1: nowhere)
+    __shared__ float scale_s[KV8_READ_ROWS * KV8_READ_THREADS / 2];
+    const int runs = hd / 8, side = KV8_READ_THREADS / runs, tile = side * KV8_READ_ROWS;
+    const int planes = k_out && v_out ? 2 * nkv : nkv;                 // which * nkv + head
+    const int plane = (int)(blockIdx.x % planes) + (k_out ? 0 : nkv);
+    const long long t0 = (long long)(blockIdx.x / planes) * tile;
     ap_pdl_trigger();
     ap_pdl_wait();
-    const long long id = (long long)blockIdx.x * KV8_THREADS + threadIdx.x;
-    const long long t = id / per_row;
-    if (t >= T) return;
-    const int item = (int)(id - t * per_row);
-    const int plane = item / runs, run = item - plane * runs;          // plane: which * nkv + head
-    TO* out = plane < nkv ? k_out : v_out;
-    if (!out) return;
-    const int pos = positions[t], seq = token_seq[t];
-    int page = -1;
-    if (pos >= 0 && pos / P < max_blocks && seq >= 0 && seq < nseq) page = block_table[(size_t)seq * max_blocks + pos / P];
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = 0.f;                           // a row without a page reads as zeros
-    if (page >= 0 && page < num_pages) {
-        const uint8_t* base = cache + (size_t)page * page_bytes;
-        const size_t row = (size_t)plane * P + pos % P;
-        const uint4 u = *reinterpret_cast<const uint4*>(base + row * hd + run * 16);
-        const float s = kv8_scale(base[(size_t)2 * nkv * P * hd + row]);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 f = kv8_unpack(w[i]);
-            x[4 * i] = f.x * s; x[4 * i + 1] = f.y * s; x[4 * i + 2] = f.z * s; x[4 * i + 3] = f.w * s;
+    for (int i = threadIdx.x; i < tile; i += KV8_READ_THREADS) {
+        long long at = -1;
+        float s = 0.f;
+        if (t0 + i < T) {
+            const int pos = positions[t0 + i], seq = token_seq[t0 + i];
+            int page = -1;
+            if (pos >= 0 && pos / P < max_blocks && seq >= 0 && seq < nseq) page = block_table[(size_t)seq * max_blocks + pos / P];
+            if (page >= 0 && page < num_pages) {
+                const size_t row = (size_t)plane * P + pos % P;
+                at = (long long)((size_t)page * page_bytes + row * hd);
+                s = kv8_scale(cache[(size_t)page * page_bytes + (size_t)2 * nkv * P * hd + row]);
+            }
         }
+        at_s[i] = at;
+        scale_s[i] = s;
     }
-    TO* dst = out + (size_t)t * nkv * hd + (size_t)(plane < nkv ? plane : plane - nkv) * hd + run * 16;
-    kv8_store8(dst, x);
-    kv8_store8(dst + 8, x + 8);
+    __syncthreads();
+    const int first = threadIdx.x / runs, col = (threadIdx.x - first * runs) * 8;
+    if (first >= side) return;                                         // (where the runs do not divide the threads)
+    uint2 u[KV8_READ_ROWS];
+#pragma unroll
+    for (int i = 0; i < KV8_READ_ROWS; ++i) {
+        const long long at = at_s[first + i * side];                   // a row without a page reads as zeros
+        u[i] = at >= 0 ? *reinterpret_cast<const uint2*>(cache + at + col) : make_uint2(0u, 0u);
+    }
+    TO* out = (plane < nkv ? k_out : v_out) + (size_t)(plane < nkv ? plane : plane - nkv) * hd + col;
+#pragma unroll
+    for (int i = 0; i < KV8_READ_ROWS; ++i) {
+        const long long t = t0 + first + i * side;
+        if (t >= T) break;
+        const float s = scale_s[first + i * side];
+        const float4 a = kv8_unpack(u[i].x), b = kv8_unpack(u[i].y);
+        TO* to = out + (size_t)t * nkv * hd;
+        kv8_store4(to, make_float4(a.x * s, a.y * s, a.z * s, a.w * s));
+        kv8_store4(to + 4, make_float4(b.x * s, b.y * s, b.z * s, b.w * s));
+    }
 }
 
 // k_out, v_out: [T][nkv][hd] of `dtype`; either may be null.
@@ -236,10 +240,11 @@ AP_EXPORT int ap_kv8_read(const void* cache, long long num_pages, long long page
     if (rc != AP_OK) return rc;
     AP_REQUIRE(((uintptr_t)k_out & 15) == 0 && ((uintptr_t)v_out & 15) == 0, "kv8_read: outputs must be 16-byte aligned");
     if (T == 0 || (!k_out && !v_out)) return AP_OK;
-    const long long threads = (long long)T * 2 * nkv * (hd / 16), ctas = (threads + KV8_THREADS - 1) / KV8_THREADS;
+    const int tile = KV8_READ_THREADS / (hd / 8) * KV8_READ_ROWS;
+    const long long ctas = ((long long)T + tile - 1) / tile * (k_out && v_out ? 2 * nkv : nkv);
     AP_REQUIRE(ctas < (1LL << 31), "kv8_read: %d rows exceed the grid", T);
 #define KV8_READ(TO)                                                                                                       \
-    AP_CHECK_PDL_LAUNCH("kv8_read", ap_launch_pdl(kv8_read_kernel<TO>, dim3((unsigned)ctas), dim3(KV8_THREADS), 0, stream,  \
+    AP_CHECK_PDL_LAUNCH("kv8_read", ap_launch_pdl(kv8_read_kernel<TO>, dim3((unsigned)ctas), dim3(KV8_READ_THREADS), 0, stream,  \
                         (const uint8_t*)cache, positions, token_seq, block_table, max_blocks, nseq, (TO*)k_out, (TO*)v_out, T, nkv, hd, P, \
                         (size_t)page_bytes, (int)num_pages))
     if (dtype == AP_F32) KV8_READ(float);
