@@ -19,38 +19,42 @@ from . import AP_BF16, AP_F32, KernelError, call, core, library, stream_handle
 _CODES = {torch.float32: AP_F32, torch.bfloat16: AP_BF16}
 
 
+@functools.lru_cache(maxsize=None)
 def kv8_page_bytes(num_kv_heads: int, page_size: int, head_dim: int) -> int:
     """Bytes of one page of one layer's 8-bit cache (numbers, scales, padding to 16)."""
     return -(-2 * num_kv_heads * page_size * (head_dim + 1) // 16) * 16
 
 
-def _take(what: str, t: torch.Tensor, name: str, dtype, dims: int, device: int) -> None:
-    if t.dtype is not dtype or t.dim() != dims or t.get_device() != device or not t.is_contiguous():
+def _take(what: str, t: torch.Tensor, name: str, dtype, dims: int, device: int):
+    """Checks a tensor; returns its shape."""
+    shape = t.shape
+    if t.dtype is not dtype or len(shape) != dims or t.get_device() != device or not t.is_contiguous():
         raise KernelError(f"{what}: {name} must be a contiguous {dims}-dimensional tensor of {dtype} on the cache's device, is "
-                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
+                          f"{tuple(shape)} {t.dtype} on {t.device}")
+    return shape
 
 
 def _take_cache(what: str, cache_layer: torch.Tensor, num_kv_heads: int, head_dim: int, page_size: int, positions: torch.Tensor,
-                token_seq: torch.Tensor, block_table: torch.Tensor) -> int:
-    """Checks the cache and the rows' metadata; returns the device."""
+                token_seq: torch.Tensor, block_table: torch.Tensor):
+    """Checks the cache and the rows' metadata; returns the device, the number of rows, what the C entry points take of the cache
+    (address, pages, bytes of one) and of the block table (address, blocks to a sequence, sequences)."""
     if head_dim <= 0 or head_dim % 16 or head_dim > 256 or num_kv_heads <= 0 or page_size <= 0:
         raise KernelError(f"{what}: {num_kv_heads} KV heads of {head_dim} in pages of {page_size} are not taken (head sizes are "
                           f"multiples of 16 up to 256)")
-    if not cache_layer.is_cuda:
-        raise KernelError(f"{what}: the cache must be a CUDA tensor")
     device = cache_layer.get_device()
-    if device != torch.cuda.current_device():
-        raise KernelError(f"{what}: the cache is on device {device}, the current device is {torch.cuda.current_device()}")
-    _take(what, cache_layer, "cache_layer", torch.uint8, 2, device)
-    if cache_layer.shape[1] != kv8_page_bytes(num_kv_heads, page_size, head_dim) or cache_layer.data_ptr() % 16:
+    if device < 0 or device != torch.cuda.current_device():
+        raise KernelError(f"{what}: the cache must be a CUDA tensor on the current device, is on {cache_layer.device}")
+    pages, page_bytes = _take(what, cache_layer, "cache_layer", torch.uint8, 2, device)
+    cache = cache_layer.data_ptr()
+    if page_bytes != kv8_page_bytes(num_kv_heads, page_size, head_dim) or cache % 16:
         raise KernelError(f"{what}: the cache must be 16-byte aligned pages of {kv8_page_bytes(num_kv_heads, page_size, head_dim)} "
                           f"bytes, is {tuple(cache_layer.shape)}")
-    _take(what, positions, "positions", torch.int32, 1, device)
-    _take(what, token_seq, "token_seq", torch.int32, 1, device)
-    _take(what, block_table, "block_table", torch.int32, 2, device)
-    if positions.shape[0] < token_seq.shape[0] or block_table.numel() == 0:
+    given, = _take(what, positions, "positions", torch.int32, 1, device)
+    T, = _take(what, token_seq, "token_seq", torch.int32, 1, device)
+    sequences, blocks = _take(what, block_table, "block_table", torch.int32, 2, device)
+    if given < T or not sequences or not blocks:
         raise KernelError(f"{what}: fewer positions than rows, or an empty block table")
-    return device
+    return device, T, (cache, pages, page_bytes), (block_table.data_ptr(), blocks, sequences)
 
 
 def rope_kv8_store(qkv: torch.Tensor, q_out: torch.Tensor, cache_layer: torch.Tensor, positions: torch.Tensor,
@@ -64,34 +68,34 @@ def rope_kv8_store(qkv: torch.Tensor, q_out: torch.Tensor, cache_layer: torch.Te
     the block table, page id outside the cache) is not kept, its query is written all the same.  A number that is not finite is kept as
     NaN.  Two rows of one step must not name the same slot."""
     what = "rope_kv8_store"
-    device = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
-    T = token_seq.shape[0]
+    device, T, cache, table = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
     width = (num_heads + 2 * num_kv_heads) * head_dim
     act, dt = _CODES.get(q_out.dtype), _CODES.get(qkv.dtype)
     if act is None or dt is None or (dt == AP_BF16 and act == AP_F32) or num_heads <= 0:
         raise KernelError(f"{what}: types {qkv.dtype} and {q_out.dtype} (float32 or bfloat16, the input no narrower than 32 bits "
                           f"where the queries are)")
-    _take(what, qkv, "qkv", torch.float32 if qkv.dim() == 3 else qkv.dtype, qkv.dim(), device)
-    _take(what, q_out, "q_out", q_out.dtype, 2, device)
-    if qkv.dim() not in (2, 3) or qkv.shape[-2] != T or qkv.shape[-1] != width or qkv.shape[0] == 0 != T or q_out.shape[0] < T \
-            or q_out.shape[1] != num_heads * head_dim:
+    S = 1
+    if qkv.dim() == 3:
+        S, rows, wide = _take(what, qkv, "qkv", torch.float32, 3, device)
+    else:
+        rows, wide = _take(what, qkv, "qkv", qkv.dtype, 2, device)
+    q_rows, q_width = _take(what, q_out, "q_out", q_out.dtype, 2, device)
+    if rows != T or wide != width or (S == 0 and T) or q_rows < T or q_width != num_heads * head_dim:
         raise KernelError(f"{what}: shapes disagree: qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)}, {T} rows of {num_heads} + "
                           f"2 x {num_kv_heads} heads of {head_dim}")
-    if qkv.data_ptr() % 16 or q_out.data_ptr() % 16:
-        raise KernelError(f"{what}: qkv and q_out must be 16-byte aligned")
-    cs = 0
+    x, q, cs = qkv.data_ptr(), q_out.data_ptr(), 0
     if cos_sin is not None:
-        _take(what, cos_sin, "cos_sin", torch.float32, 3, device)
-        if cos_sin.shape[0] < T or cos_sin.shape[1] != head_dim // 2 or cos_sin.shape[2] != 2 or cos_sin.data_ptr() % 16:
-            raise KernelError(f"{what}: cos_sin must be 16-byte aligned [T, head_dim/2, 2], is {tuple(cos_sin.shape)}")
+        angles, pairs, two = _take(what, cos_sin, "cos_sin", torch.float32, 3, device)
         cs = cos_sin.data_ptr()
+        if angles < T or pairs != head_dim // 2 or two != 2:
+            raise KernelError(f"{what}: cos_sin must be [T, head_dim/2, 2], is {tuple(cos_sin.shape)}")
+    if (x | q | cs) % 16:
+        raise KernelError(f"{what}: qkv, q_out and cos_sin must be 16-byte aligned")
     if pairing not in (0, 1, 2):
         raise KernelError(f"{what}: unknown pairing {pairing}")
-    S = qkv.shape[0] if qkv.dim() == 3 else 1
-    call(core(), "ap_rope_kv8_store", qkv.data_ptr(), dt, S, T * width, q_out.data_ptr(), act, cache_layer.data_ptr(),
-         cache_layer.shape[0], cache_layer.shape[1], positions.data_ptr(), token_seq.data_ptr(), block_table.data_ptr(),
-         block_table.shape[1], block_table.shape[0], cs, int(pairing), T, num_heads, num_kv_heads, head_dim, page_size,
-         stream_handle())
+    if T:
+        call(core(), "ap_rope_kv8_store", x, dt, S, T * width, q, act, *cache, positions.data_ptr(), token_seq.data_ptr(), *table, cs,
+             int(pairing), T, num_heads, num_kv_heads, head_dim, page_size, stream_handle())
 
 
 def kv8_read(cache_layer: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor, block_table: torch.Tensor,
@@ -101,24 +105,24 @@ def kv8_read(cache_layer: torch.Tensor, positions: torch.Tensor, token_seq: torc
     None) gets position ``positions[r]`` of sequence ``token_seq[r]``, exactly what the cache stands for (bfloat16 holds it too).
     A row without a page reads as zeros."""
     what = "kv8_read"
-    device = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
-    T = token_seq.shape[0]
+    device, T, cache, table = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
     some = k_out if k_out is not None else v_out
     if some is None:
         return
-    code = _CODES.get(some.dtype)
+    dtype, width = some.dtype, num_kv_heads * head_dim
+    code = _CODES.get(dtype)
     if code is None:
-        raise KernelError(f"{what}: outputs of {some.dtype} are not taken (float32, bfloat16)")
+        raise KernelError(f"{what}: outputs of {dtype} are not taken (float32, bfloat16)")
     ptr = [0, 0]
     for i, t in enumerate((k_out, v_out)):
         if t is not None:
-            _take(what, t, "an output", some.dtype, 2, device)
-            if t.shape[0] < T or t.shape[1] != num_kv_heads * head_dim or t.data_ptr() % 16:
-                raise KernelError(f"{what}: outputs must be 16-byte aligned [rows, {num_kv_heads * head_dim}], one is {tuple(t.shape)}")
+            rows, wide = _take(what, t, "an output", dtype, 2, device)
             ptr[i] = t.data_ptr()
-    call(core(), "ap_kv8_read", cache_layer.data_ptr(), cache_layer.shape[0], cache_layer.shape[1], positions.data_ptr(),
-         token_seq.data_ptr(), block_table.data_ptr(), block_table.shape[1], block_table.shape[0], ptr[0], ptr[1], code, T,
-         num_kv_heads, head_dim, page_size, stream_handle())
+            if rows < T or wide != width or ptr[i] % 16:
+                raise KernelError(f"{what}: outputs must be 16-byte aligned [rows, {width}], one is {tuple(t.shape)}")
+    if T:
+        call(core(), "ap_kv8_read", *cache, positions.data_ptr(), token_seq.data_ptr(), *table, *ptr, code, T, num_kv_heads, head_dim,
+             page_size, stream_handle())
 
 
 _nonces = itertools.count(random.getrandbits(61))
@@ -156,24 +160,26 @@ def _scratch_bytes(num_heads: int, num_kv_heads: int, head_dim: int, ctas: int) 
     return library.attention(head_dim).ap_attention_kv8_decode_scratch(num_heads, num_kv_heads, ctas)
 
 
-def _rows(q, out, cache_layer, block_table, token_seq, positions, first, rows, num_heads, num_kv_heads, head_dim, page_size, scale,
-          window, longest, mean, scratch, device) -> None:
-    """Rows ``first`` to ``first + rows`` one by one, up to ``longest`` keys to a row and some ``mean``."""
+def _rows(q, out, cache, table, token_seq, positions, rows, num_heads, num_kv_heads, head_dim, page_size, scale, window, longest, mean,
+          scratch, device) -> None:
+    """The first ``rows`` rows one by one, up to ``longest`` keys to a row and some ``mean``."""
     lib = library.attention(head_dim)
-    group = num_heads // num_kv_heads
     if window:
         longest, mean = min(longest, window + 64), min(mean, window + 64)
-    step = 512
-    for r in range(first, first + rows, step):
-        n = min(step, first + rows - r)
-        ctas, cluster = plan_rows(n * num_kv_heads * -(-group // 8), -(-longest // 64), -(-mean // 64), _sms(device))
-        need = 0 if cluster else _scratch_bytes(num_heads, num_kv_heads, head_dim, ctas)
-        buf = None if cluster else scratch("attn.kv8", (need // 4,), torch.float32) if scratch is not None else \
-            torch.empty(need // 4, dtype=torch.float32, device=q.device)
-        call(lib, "ap_attention_kv8_decode", q.data_ptr() + 2 * r * q.shape[1], out.data_ptr() + 2 * r * q.shape[1],
-             cache_layer.data_ptr(), cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr(), block_table.shape[1],
-             block_table.shape[0], token_seq.data_ptr() + 4 * r, positions.data_ptr() + 4 * r, n, num_heads, num_kv_heads, head_dim,
-             page_size, float(scale), int(window), ctas, cluster, buf.data_ptr() if buf is not None else 0, need, next(_nonces) % (1 << 62) + 1, stream_handle())
+    step, sets = 512, num_kv_heads * -(-(num_heads // num_kv_heads) // 8)
+    x, y, seq, pos, width = q.data_ptr(), out.data_ptr(), token_seq.data_ptr(), positions.data_ptr(), num_heads * head_dim
+    for r in range(0, rows, step):
+        n = min(step, rows - r)
+        ctas, cluster = plan_rows(n * sets, -(-longest // 64), -(-mean // 64), _sms(device))
+        at, need = 0, 0
+        if not cluster:
+            need = _scratch_bytes(num_heads, num_kv_heads, head_dim, ctas)
+            buf = scratch("attn.kv8", (need // 4,), torch.float32) if scratch is not None else \
+                torch.empty(need // 4, dtype=torch.float32, device=q.device)
+            at = buf.data_ptr()
+        call(lib, "ap_attention_kv8_decode", x + 2 * r * width, y + 2 * r * width, *cache, *table, seq + 4 * r, pos + 4 * r, n,
+             num_heads, num_kv_heads, head_dim, page_size, float(scale), int(window), ctas, cluster, at, need,
+             next(_nonces) % (1 << 62) + 1, stream_handle())
 
 
 @functools.lru_cache(maxsize=None)
@@ -209,11 +215,11 @@ def plan_portions(query_lens: Sequence[int], per_tile: int, num_kv_heads: int, k
 WIDE_SCRATCH = 1 << 30
 
 
-def _portions(q, out, cache_layer, block_table, seq_start, positions, first_seq, query_lens, T, num_heads, num_kv_heads, head_dim,
-              page_size, scale, window, per_tile, longest, scratch, device) -> None:
+def _portions(q, out, cache, table, seq_start, positions, first_seq, query_lens, T, num_heads, num_kv_heads, head_dim, page_size, scale,
+              window, per_tile, longest, scratch, device) -> None:
     """The sequences from ``first_seq`` on, by their ``query_lens``, of up to ``longest`` keys; their rows follow those of the sequences
     before."""
-    width, lib = block_table.shape[1], library.attention(head_dim)
+    (blocks, width, _), lib = table, library.attention(head_dim)
     one = lib.ap_attention_kv8_tcgen05_scratch(1, width, page_size, num_kv_heads)
     step = max(1, min(len(query_lens), WIDE_SCRATCH // one))
     buf = scratch("attn.kv8_wide", (step * one // 2,), torch.bfloat16) if scratch is not None else \
@@ -223,8 +229,7 @@ def _portions(q, out, cache_layer, block_table, seq_start, positions, first_seq,
         lens = query_lens[at:at + step]
         query_tiles, ctas, slices = plan_portions(lens, per_tile, num_kv_heads, longest - max(lens) // 2, _sms(device))
         if ctas:
-            call(lib, "ap_attention_kv8_tcgen05", q.data_ptr(), out.data_ptr(), cache_layer.data_ptr(), cache_layer.shape[0],
-                 cache_layer.shape[1], block_table.data_ptr() + 4 * (first_seq + at) * width, width,
+            call(lib, "ap_attention_kv8_tcgen05", q.data_ptr(), out.data_ptr(), *cache, blocks + 4 * (first_seq + at) * width, width,
                  seq_start.data_ptr() + 4 * (first_seq + at), positions.data_ptr(), len(lens), T, num_heads, num_kv_heads, head_dim,
                  page_size, float(scale), int(window), query_tiles, ctas, slices, buf.data_ptr(), step * one, stream_handle())
 
@@ -239,40 +244,40 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
     before its position (the last ``window`` of them, 0: all) whose page is there; one that sees none gets zeros.  The rows of a
     sequence follow one another and so do their positions."""
     what = "attention_kv8"
-    device = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
-    T = token_seq.shape[0]
+    device, T, cache, table = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
     code = _CODES.get(q.dtype)
     if code is None or num_heads <= 0 or num_heads % num_kv_heads or window < 0:
         raise KernelError(f"{what}: {num_heads} heads on {num_kv_heads} KV heads in {q.dtype}, window {window}")
-    _take(what, q, "q", q.dtype, 2, device)
-    _take(what, out, "out", q.dtype, 2, device)
-    if q.shape[0] < T or q.shape[1] != num_heads * head_dim or out.shape != q.shape or q.data_ptr() % 16 or out.data_ptr() % 16:
+    rows, width = shape = _take(what, q, "q", q.dtype, 2, device)
+    if _take(what, out, "out", q.dtype, 2, device) != shape or rows < T or width != num_heads * head_dim \
+            or (q.data_ptr() | out.data_ptr()) % 16:
         raise KernelError(f"{what}: q {tuple(q.shape)} and out {tuple(out.shape)} must be 16-byte aligned rows of {num_heads} heads of "
                           f"{head_dim}, {T} at least")
-    if seq_start is not None and query_lens is not None:
-        _take(what, seq_start, "seq_start", torch.int32, 1, device)
-        if seq_start.shape[0] != len(query_lens) + 1 or sum(query_lens) != T or block_table.shape[0] < len(query_lens):
+    by_sequence = seq_start is not None and query_lens is not None
+    if by_sequence:
+        starts, = _take(what, seq_start, "seq_start", torch.int32, 1, device)
+        if starts != len(query_lens) + 1 or sum(query_lens) != T or table[2] < len(query_lens):
             raise KernelError(f"{what}: seq_start, query_lens and the block table do not describe the rows")
-    if code == AP_BF16 and T and 0 < cache_layer.numel() < 1 << 36 and _single_rows_taken(head_dim, page_size):
+    if not T:
+        return
+    if code == AP_BF16 and 0 < cache[1] * cache[2] < 1 << 36 and _single_rows_taken(head_dim, page_size):
         # sequences that bring one row each, then portions (one-row sequences further back ride along with them)
-        widest = block_table.shape[1] * page_size
+        widest = table[1] * page_size
         ones, rows = 0, T
-        if query_lens is not None and seq_start is not None:
+        if by_sequence:
             while ones < len(query_lens) and query_lens[ones] == 1:
                 ones += 1
             if ones < len(query_lens):
                 per_tile = _portions_taken(num_heads, num_kv_heads, head_dim, page_size) if scale > 0 else 0
                 if per_tile:
-                    _portions(q, out, cache_layer, block_table, seq_start, positions, ones, query_lens[ones:], T, num_heads,
-                              num_kv_heads, head_dim, page_size, scale, window, per_tile, max_context if max_context and not ones else widest,
-                              scratch, device)
+                    _portions(q, out, cache, table, seq_start, positions, ones, query_lens[ones:], T, num_heads, num_kv_heads, head_dim,
+                              page_size, scale, window, per_tile, max_context if max_context and not ones else widest, scratch, device)
                     rows = ones
         if rows:
             longest = max_context if max_context and rows == ones else widest
-            _rows(q, out, cache_layer, block_table, token_seq, positions, 0, rows, num_heads, num_kv_heads, head_dim, page_size, scale,
-                  window, longest, min(mean_context or longest, longest), scratch, device)
+            _rows(q, out, cache, table, token_seq, positions, rows, num_heads, num_kv_heads, head_dim, page_size, scale, window,
+                  longest, min(mean_context or longest, longest), scratch, device)
         return
-    call(library.attention(head_dim), "ap_attention_kv8_rows", q.data_ptr(), out.data_ptr(), code, cache_layer.data_ptr(),
-         cache_layer.shape[0], cache_layer.shape[1], block_table.data_ptr(), block_table.shape[1], block_table.shape[0],
+    call(library.attention(head_dim), "ap_attention_kv8_rows", q.data_ptr(), out.data_ptr(), code, *cache, *table,
          token_seq.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, head_dim, page_size, float(scale), int(window),
          stream_handle())

@@ -34,13 +34,13 @@ _CORE_SIGNATURES = {
     "ap_norm_residual": [_P, _P, _I, _L, _P, _I, _F, _F, _P, _I, _I, _I, _P],
     "ap_swiglu": [_P, _I, _I, _L, _P, _I, _I, _I, _I, _P],
     "ap_gemm_simt": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _L, _L, _L, _P],
-    # int ap_stage_step(host, dev, first, n, device_tokens, off_tokens, tokens, index, stream)
     # int ap_rope_kv8_store(in, in_dtype, S, in_stride, q_out, act_dtype, cache, num_pages, page_bytes, positions, token_seq,
     #                       block_table, max_blocks, nseq, cos_sin, pairing, T, nh, nkv, hd, P, stream)
     "ap_rope_kv8_store": [_P, _I, _I, _L, _P, _I, _P, _L, _L, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _P],
     # int ap_kv8_read(cache, num_pages, page_bytes, positions, token_seq, block_table, max_blocks, nseq, k_out, v_out, dtype, T,
     #                 nkv, hd, P, stream)
     "ap_kv8_read": [_P, _L, _L, _P, _P, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P],
+    # int ap_stage_step(host, dev, first, n, device_tokens, off_tokens, tokens, index, stream)
     "ap_stage_step": [_P, _P, _I, _I, _P, _I, _I, _P, _P],
     "ap_argmax": [_P, _L, _I, _I, _P, _P, _P],
     "ap_sample": [_P, _L, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P],
