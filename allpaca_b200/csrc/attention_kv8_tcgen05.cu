@@ -74,7 +74,7 @@ struct AttnT8Params {
 // What the rows of sequence s see: tiles t_lo .. t_hi of its keys (none: t_hi < t_lo), keys kmin .. kmax
 __device__ __forceinline__ void t8_span(const int* positions, int row0, int ntok, int window, int last_key, int& kmin, int& kmax) {
     kmax = min(positions[row0 + ntok - 1], last_key);
-    const int first = positions[row0];
+    const int first = min(positions[row0], last_key);
     kmin = (window > 0 && first - window + 1 > 0) ? first - window + 1 : 0;
 }
 
@@ -362,7 +362,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         const uint32_t lane_base = tmem_base + ((uint32_t)(qtr * 32) << 16);
         const uint32_t s_cols = lane_base + (uint32_t)(x * BKV);
         const uint32_t o_cols = lane_base + (uint32_t)(kOCol + x * HD);
-        const int qpos = p.positions[row0 + (rvalid ? tok : 0)];
+        const int qpos = min(p.positions[row0 + (rvalid ? tok : 0)], p.max_blocks * p.P - 1);
         float mref = -INFINITY, l = 0.f;               // the row's reference maximum (log2 units) and sum
         bool ok = true;                                // the same in all lanes of a warp
         int page = page_of(0);
