@@ -7,6 +7,14 @@
 // With key j kept as codes c_j and scale 2^a_j, value j as d_j and 2^b_j:
 //   s_j = scale * 2^a_j * (q . c_j),   out = sum_j exp(s_j - m) 2^b_j d_j / sum_j exp(s_j - m).
 //
+// A CTA takes a row of one query head and walks its keys K8_CHUNK at a time, a key to a thread for the scores, a column of four to
+// a thread for the values, with the running maximum and sum of a softmax.  It is here for float32 activations, whose products no
+// tensor core takes in full, and for what the kernels of bfloat16 rows and portions refuse (pages of other sizes, caches of 64 GB and more):
+// it reads a KV head's keys once for every query head and row, so arithmetic and L2 bound it, not the 8-bit keys' bytes (4 float32 rows of
+// 32 heads of 64 with 20 to 700 keys: 10.0 us, floor 0.5; 64 rows of 2000 keys, heads of 128: 250, floor 42).  The chunks of a row wait for
+// one another, hence many keys to a chunk: with 128 threads the two take 15.9 and 309 us, with 512 9.5 and 319; a prompt of 499
+// rows takes 131 us, 117 with 128 threads, 182 with 512.
+//
 // Reference counterparts: attention_qtile_kernel and attention_split_gqa_kernel (cuda/src/kernels.cu:1801, :1874), the causal
 // rule :1583-1585; the reference's keys and values are 32-bit.
 #include "kv8.cuh"
@@ -18,8 +26,8 @@
 #endif
 
 #define HD AP_HEAD_DIM
-#define K8_THREADS 128
-#define K8_CHUNK 128
+#define K8_THREADS 256
+#define K8_CHUNK K8_THREADS                               // keys at a time: one to a thread
 #define K8_LANES (HD / 4 < K8_THREADS ? HD / 4 : K8_THREADS)     // threads side by side on a value row, four numbers each
 #define K8_GROUPS (K8_THREADS / K8_LANES)
 
