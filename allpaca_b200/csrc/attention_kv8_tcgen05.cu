@@ -85,8 +85,9 @@ kv8_widen_kernel(const uint8_t* __restrict__ cache, size_t page_bytes, const Att
     __shared__ long long at_s[BKV];                       // where a key's numbers lie (-1: nowhere)
     __shared__ float scale_s[BKV];
     const int s = blockIdx.z, plane = blockIdx.y, t = blockIdx.x;
-    ap_pdl_trigger();
+    // the second kernel may start once everything before this one has ended: it reads all but this one's result ahead of its own wait
     ap_pdl_wait();
+    ap_pdl_trigger();
     const int row0 = p.seq_start[s], ntok = p.seq_start[s + 1] - row0;
     if (ntok <= 0) return;
     int kmin, kmax;
@@ -191,7 +192,6 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         reinterpret_cast<uint4*>(smem + Smem::kQ + Q_BYTES)[i] = make_uint4(0, 0, 0, 0);
     tc::fence_proxy_async();
     if (warp == kMmaWarp) tc::tmem_alloc(tmem_slot, T8_TMEM_COLS(NX));
-    ap_pdl_wait();
     if (warp == 0) {
         // late portions of a sequence have the most keys to walk: hand them out first
         // (the KV head is the fast index of the grid: all heads of the longest portions start first)
@@ -234,6 +234,8 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         head0 = kvh * G;
     }
     const bool has_b = NX == 2 && ntok > p.tokens_per_tile;          // the second query tile holds rows
+    // Where there is no second tile its place takes every other key tile of the first one's rows, as one more slice
+    const bool halves = SPLIT && NX == 2 && !has_b;
     if (active) {
         t8_span(p.positions, row0, ntok, p.window, p.max_blocks * p.P - 1, kmin, kmax);
     }
@@ -260,13 +262,16 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     if (NX == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == kLoadWarp) {
-        if (active && ntiles > 0) {
+        if (!(active && ntiles > 0)) {
+            ap_pdl_wait();                                 // (no CTA ends before the widening has)
+        } else {
             if (lane == 0) {
                 tc::mbar_expect_tx(q_full, (uint32_t)((has_b ? 2 : 1) * Q_BYTES));
                 for (int x = 0; x < (has_b ? 2 : 1); ++x)
                     for (int h = 0; h < NHALF; ++h)
                         tc::tma_load_3d(smem + Smem::kQ + x * Q_BYTES + h * SUB_BYTES, &tmap_q, h * 64, head0,
                                         row0 + x * p.tokens_per_tile, q_full);
+                ap_pdl_wait();                             // the widened keys and values
                 const int k_row = (seq * 2 * p.nkv + kvh) * p.cap + t_lo * BKV, v_row = k_row + p.nkv * p.cap;
                 auto load = [&](int it, int row, uint64_t* full, uint64_t* free, int base) -> bool {
                     const int s = it % kStages;
@@ -297,10 +302,11 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             const int nx = has_b ? 2 : 1;
             // S_x = Q_x K^T of key tile `it`
             auto scores = [&](int it, int x) {
+                const int of = halves ? 0 : x;
                 const int s = it % kStages;
 #pragma unroll
                 for (int h = 0; h < NHALF; ++h) {
-                    const uint64_t qd = tc::smem_desc_k_major_sw128(smem + Smem::kQ + x * Q_BYTES + h * SUB_BYTES);
+                    const uint64_t qd = tc::smem_desc_k_major_sw128(smem + Smem::kQ + of * Q_BYTES + h * SUB_BYTES);
                     const uint64_t kd = tc::smem_desc_k_major_sw128(smem + Smem::kK + s * KV_BYTES + h * SUB_BYTES);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -308,31 +314,59 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                 }
                 tc::mma_commit(&s_full[x]);
             };
+            // O_x += P_x V of key tile `it`, the first of x's or not
+            auto values = [&](int it, int x, bool first) {
+                const uint64_t vd = tc::smem_desc_mn_major_sw128(smem + Smem::kV + it % kStages * KV_BYTES, SUB_BYTES);
+                const uint32_t pt = tmem_base + (uint32_t)(x * BKV);      // P_x lies over S_x
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks)
+                    tc::mma_bf16_a_tmem(tmem_base + (uint32_t)(kOCol + x * HD), pt + (uint32_t)(ks * 8),
+                                        vd + (uint64_t)(ks * (16 * 128 / 16)), idesc_o, (!first || ks > 0) ? 1u : 0u);
+            };
             bool ok = tc::mbar_wait(q_full, 0);
-            if (ok) ok = tc::mbar_wait(&k_full[0], 0);
-            if (ok) {
+            if (halves) {
+                // two chains of their own: tile `it` is x = it % 2's, and so are its stages
+                for (int x = 0; x < 2 && x < ntiles && ok; ++x) {
+                    ok = tc::mbar_wait(&k_full[x], 0);
+                    if (!ok) break;
+                    tc::fence_after_sync();
+                    scores(x, x);
+                    tc::mma_commit(&k_free[x]);
+                }
+                for (int it = 0; it < ntiles && ok; ++it) {
+                    const int x = it & 1;
+                    const uint32_t ph = (uint32_t)((it >> 1) & 1);
+                    const bool more = it + 2 < ntiles;
+                    ok = tc::mbar_wait(&v_full[x], ph) && (!more || tc::mbar_wait(&k_full[x], ph ^ 1u)) && tc::mbar_wait(&p_ready[x], ph);
+                    if (!ok || *abort_flag) break;
+                    tc::fence_after_sync();
+                    values(it, x, it < 2);
+                    tc::mma_commit(more ? &v_free[x] : &o_full[x]);
+                    if (more) {
+                        scores(it + 2, x);
+                        tc::mma_commit(&k_free[x]);
+                    }
+                }
+            }
+            if (ok && !halves) ok = tc::mbar_wait(&k_full[0], 0);
+            if (ok && !halves) {
                 tc::fence_after_sync();
                 for (int x = 0; x < nx; ++x) scores(0, x);
                 tc::mma_commit(&k_free[0]);
             }
-            for (int it = 0; it < ntiles && ok; ++it) {
+            for (int it = 0; it < ntiles && ok && !halves; ++it) {
                 const int sv = it % kStages, sk = (it + 1) % kStages;
                 const bool more = it + 1 < ntiles;
                 ok = tc::mbar_wait(&v_full[sv], (uint32_t)((it / kStages) & 1)) &&
                      (!more || tc::mbar_wait(&k_full[sk], (uint32_t)(((it + 1) / kStages) & 1)));
                 if (!ok || *abort_flag) break;
-                const uint64_t vd = tc::smem_desc_mn_major_sw128(smem + Smem::kV + sv * KV_BYTES, SUB_BYTES);
                 for (int x = 0; x < nx && ok; ++x) {
                     // O_x += P_x V as soon as the tile's group has written P_x (and scaled O_x down where a row's reference
                     // maximum moved); then S_x of the next key tile, which the group turns to while the other tile's products run
                     ok = tc::mbar_wait(&p_ready[x], (uint32_t)(it & 1));
                     if (!ok) break;
                     tc::fence_after_sync();
-                    const uint32_t pt = tmem_base + (uint32_t)(x * BKV);      // P_x lies over S_x
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)
-                        tc::mma_bf16_a_tmem(tmem_base + (uint32_t)(kOCol + x * HD), pt + (uint32_t)(ks * 8),
-                                            vd + (uint64_t)(ks * (16 * 128 / 16)), idesc_o, (it > 0 || ks > 0) ? 1u : 0u);
+                    values(it, x, it == 0);
                     if (!more) tc::mma_commit(&o_full[x]);
                     if (NX == 1) tc::mma_commit(&v_free[sv]);
                     if (more) scores(it + 1, x);
@@ -352,12 +386,13 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     } else {
     if (NX == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    if (active && (warp < 4 || has_b)) {
+    if (active && (warp < 4 || has_b || halves)) {
         // ---- softmax: warps 0..3 own query tile a, warps 4..7 tile b; one row per thread ----
         const int x = warp >> 2;
         const int qtr = warp & 3;
         const int r = qtr * 32 + lane;                 // row of the tile = (token r / G, head r % G)
-        const int tok = x * p.tokens_per_tile + r / G, hq = r % G;
+        const int tok = (halves ? 0 : x * p.tokens_per_tile) + r / G, hq = r % G;
+        const int it0 = halves ? x : 0, step = halves ? 2 : 1;         // the key tiles of this query tile
         const bool rvalid = tok < ntok;
         const uint32_t lane_base = tmem_base + ((uint32_t)(qtr * 32) << 16);
         const uint32_t s_cols = lane_base + (uint32_t)(x * BKV);
@@ -365,14 +400,15 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         const int qpos = min(p.positions[row0 + (rvalid ? tok : 0)], p.max_blocks * p.P - 1);
         float mref = -INFINITY, l = 0.f;               // the row's reference maximum (log2 units) and sum
         bool ok = true;                                // the same in all lanes of a warp
-        int page = page_of(0);
-        for (int it = 0; it < ntiles; ++it) {
+        int page = page_of(it0);
+        uint32_t ph = 0;
+        for (int it = it0; it < ntiles; it += step, ph ^= 1u) {
             const int k0 = (t_lo + it) * BKV;
             // pages that are not there (rare: a caller gives them back behind a window)
             const uint32_t gone = __ballot_sync(0xffffffffu, page < 0);
-            page = page_of(it + 1);
+            page = page_of(it + step);
             // tcgen05.ld and .st are warp-wide instructions: whatever decides whether one runs is a vote
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_full[x], (uint32_t)(it & 1)))) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_full[x], ph))) { ok = false; break; }
             tc::fence_after_sync();
             // (rows that are none see everything: their sums go nowhere)
             const bool row_all = !rvalid || (k0 + BKV - 1 <= qpos && (p.window <= 0 || qpos - k0 < p.window));
@@ -423,7 +459,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                     mref = mx;
                     l *= alpha;
                 }
-                if (it > 0 && __any_sync(0xffffffffu, grow)) {
+                if (it > it0 && __any_sync(0xffffffffu, grow)) {
                     // scale this warp's rows of O_x down.  The product of the tile before into O_x is in: it was issued before the
                     // scores whose arrival (s_full) this warp has seen, and an arrival stands for everything issued before it
 #pragma unroll 1
@@ -460,7 +496,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             if (lane == 0) tc::mbar_arrive(&p_ready[x]);
         }
         // the last product into O_x, then the row goes out, or to the other slices
-        if (ok && ntiles > 0 && !__all_sync(0xffffffffu, tc::mbar_wait(&o_full[x], 0))) ok = false;
+        if (ok && ntiles > it0 && !__all_sync(0xffffffffu, tc::mbar_wait(&o_full[x], 0))) ok = false;
         tc::fence_after_sync();
         if (!ok) {
             if (!*abort_flag) {
@@ -470,12 +506,12 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         } else if (SPLIT) {
             // (both query tiles' products are done when this one's are only where there is no other: wait for it before its operands are
             // written over)
-            if (has_b && ntiles > 0 && !__all_sync(0xffffffffu, tc::mbar_wait(&o_full[x ^ 1], 0))) ok = false;
+            if ((has_b || halves) && ntiles > (halves ? x ^ 1 : 0) && !__all_sync(0xffffffffu, tc::mbar_wait(&o_full[x ^ 1], 0))) ok = false;
             float* sums = reinterpret_cast<float*>(smem + Smem::kSums) + (size_t)(x * BQ + r) * T8_PITCH;
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 uint32_t w[32];
-                if (ntiles > 0) {
+                if (ntiles > it0) {
                     tc::tmem_ld_x32(o_cols + (uint32_t)c, w);
                     tc::tmem_ld_wait();
                 } else {
@@ -533,14 +569,15 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                 L[e] = 0.f;
                 O[e] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            for (int z = 0; z < ns; ++z) {
+            for (int z2 = 0; z2 < (halves ? 2 * ns : ns); ++z2) {
+                const uint32_t z = (uint32_t)(halves ? z2 >> 1 : z2), half = (uint32_t)(halves ? z2 & 1 : 0);
                 float m[kAtOnce], l[kAtOnce];
                 float4 o[kAtOnce];
 #pragma unroll
                 for (int e = 0; e < kAtOnce; ++e) {
-                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[e]), "=f"(l[e]) : "r"(tc::map_to_rank(stats[e], (uint32_t)z)));
+                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[e]), "=f"(l[e]) : "r"(tc::map_to_rank(stats[e] + half * (BQ * 8), z)));
                     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                 : "=f"(o[e].x), "=f"(o[e].y), "=f"(o[e].z), "=f"(o[e].w) : "r"(tc::map_to_rank(sums[e], (uint32_t)z)));
+                                 : "=f"(o[e].x), "=f"(o[e].y), "=f"(o[e].z), "=f"(o[e].w) : "r"(tc::map_to_rank(sums[e] + half * (BQ * T8_PITCH * 4), z)));
                 }
 #pragma unroll
                 for (int e = 0; e < kAtOnce; ++e) {
