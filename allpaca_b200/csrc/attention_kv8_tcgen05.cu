@@ -11,7 +11,12 @@
 // Widening first costs 6 bytes of traffic to a number, half of it in L2 where the keys fit there.  Widening inside the second kernel, every
 // tile in every CTA that reads it, was built and measured: four to six warps needed 3400 to 5100 cycles to a key tile, loading a box to
 // a page 4400, where the products and the softmax need 3700: 1470 us for 2048 rows behind 30000 keys (1.2 TFLOP), the two
-// kernels 1015; 17 rows behind 8191 keys 39 us, the two kernels 37.
+// kernels 1015; 17 rows behind 8191 keys 39 us, the two kernels 31.
+//
+// A query tile without a second one beside it (few rows) walks two key tiles at once, each half of the CTA its own: 17 rows behind 32000
+// keys 80 us, one by one 104.  2048 rows behind 30000 keys run at 1.2 PFLOP/s, 0.73 of the measured peak of a dense bfloat16 product, bound by
+// the softmax (exponentials, and the scores' way through registers) beside the products; few rows by the way from one key tile
+// to the next (2 us for two of them), the widening (6 us of 31 behind 8191 keys, 31 of 80 behind 32000) and the slices' meeting (7).
 //
 // Few rows leave most SMs idle: then the keys are cut into slices, a cluster of 2, 4 or 8 CTAs works on one set of rows, and the slices'
 // sums are added up through distributed shared memory, every CTA taking its share of the rows.  One launch, no scratch.
@@ -256,6 +261,9 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         return page < p.num_pages ? page : -1;
     };
 
+    float mref = -INFINITY, l = 0.f;                   // a softmax thread's row: its reference maximum (log2 units) and sum
+    bool ok = true;                                    // the same in all lanes of a warp
+
     // Registers move from the warps that only issue copies and products to the softmax warps, which hold a row of 128 scores each (the
     // unit of such a move is four warps): 2 x 224 + 56 = 504 to a thread of each, or 192 + 64 = 256, what the launch holds.
     if (warp >= kLoadWarp) {
@@ -323,7 +331,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                     tc::mma_bf16_a_tmem(tmem_base + (uint32_t)(kOCol + x * HD), pt + (uint32_t)(ks * 8),
                                         vd + (uint64_t)(ks * (16 * 128 / 16)), idesc_o, (!first || ks > 0) ? 1u : 0u);
             };
-            bool ok = tc::mbar_wait(q_full, 0);
+            ok = tc::mbar_wait(q_full, 0);
             if (halves) {
                 // two chains of their own: tile `it` is x = it % 2's, and so are its stages
                 for (int x = 0; x < 2 && x < ntiles && ok; ++x) {
@@ -398,8 +406,6 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         const uint32_t s_cols = lane_base + (uint32_t)(x * BKV);
         const uint32_t o_cols = lane_base + (uint32_t)(kOCol + x * HD);
         const int qpos = min(p.positions[row0 + (rvalid ? tok : 0)], p.max_blocks * p.P - 1);
-        float mref = -INFINITY, l = 0.f;               // the row's reference maximum (log2 units) and sum
-        bool ok = true;                                // the same in all lanes of a warp
         int page = page_of(it0);
         uint32_t ph = 0;
         for (int it = it0; it < ntiles; it += step, ph ^= 1u) {
@@ -504,25 +510,8 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                 atomicExch(&g_t8_status, T8_ERR_WAIT);
             }
         } else if (SPLIT) {
-            // (both query tiles' products are done when this one's are only where there is no other: wait for it before its operands are
-            // written over)
-            if ((has_b || halves) && ntiles > (halves ? x ^ 1 : 0) && !__all_sync(0xffffffffu, tc::mbar_wait(&o_full[x ^ 1], 0))) ok = false;
-            float* sums = reinterpret_cast<float*>(smem + Smem::kSums) + (size_t)(x * BQ + r) * T8_PITCH;
-#pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-                uint32_t w[32];
-                if (ntiles > it0) {
-                    tc::tmem_ld_x32(o_cols + (uint32_t)c, w);
-                    tc::tmem_ld_wait();
-                } else {
-#pragma unroll
-                    for (int d = 0; d < 32; ++d) w[d] = 0u;
-                }
-#pragma unroll
-                for (int d = 0; d < 32; d += 4)
-                    *reinterpret_cast<uint4*>(sums + c + d) = make_uint4(w[d], w[d + 1], w[d + 2], w[d + 3]);
-            }
-            *reinterpret_cast<float2*>(smem + Smem::kStats + (x * BQ + r) * 8) = make_float2(mref, l);
+            // (this tile's products may be done before the other's, whose operands the sums are about to lie over)
+            if ((has_b || halves) && ntiles > (halves ? x ^ 1 : 0)) ok = __all_sync(0xffffffffu, tc::mbar_wait(&o_full[x ^ 1], 0));
         } else {
             const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;     // (a sum that is not a number stays one)
             bf16* dst = p.out + ((size_t)(row0 + (rvalid ? tok : 0)) * p.nh + head0 + hq) * HD;
@@ -552,56 +541,76 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     }
     }
     if (SPLIT) {
-        // Rows' sums of all slices, added up in the slices' order: row i of the CTAs' rows by CTA i % nsplit, four numbers to a thread
+        // The slices' sums meet in CTA i % nsplit for row i, over the tiles (the cluster's products are all done): every thread sends its
+        // row there (halves: source 2 z + x is tile x of slice z).  Then a thread to a row turns its sources' maxima and sums into weights,
+        // and all threads add up, four numbers each, in the sources' order.  3.2 us to send and 2 to add for 17 rows of 4 heads, 4 and 4 for
+        // 512 rows in two slices: barriers and code that runs for the first time, not bytes (unrolled four times it adds no faster,
+        // a row to a warp at a time, 10 us).
+        const int ns = p.nsplit, shift = __ffs(ns) - 1, rank = (int)blockIdx.y, x = warp >> 2;
+        const int sources = halves ? 2 * ns : ns, rows = (halves ? BQ : NX * BQ) >> shift;       // rows of a source that meet here
         tc::cluster_sync();
-        const int ns = p.nsplit, rank = (int)blockIdx.y, mine = (ntok * G - rank + ns - 1) / ns;
-        constexpr int kAtOnce = 4;
-        for (int k0 = threadIdx.x; warp < kLoadWarp && k0 < mine * (HD / 4); k0 += kAtOnce * NX * 128) {
-            uint32_t stats[kAtOnce], sums[kAtOnce];
-            float M[kAtOnce], L[kAtOnce];
-            float4 O[kAtOnce];
+        if (warp < kLoadWarp && active && (warp < 4 || has_b || halves)) {
+            const int r = (warp & 3) * 32 + lane, i = halves ? r : x * BQ + r;
+            const uint32_t o_cols = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(kOCol + x * HD);
+            const int slot = (halves ? 2 * rank + x : rank) * rows + (i >> shift);
+            const uint32_t to = (uint32_t)(i & (ns - 1));
+            const uint32_t sums = tc::map_to_rank(tc::smem_addr(smem + Smem::kSums) + (uint32_t)(slot * T8_PITCH) * 4u, to);
+            const uint32_t stats = tc::map_to_rank(tc::smem_addr(smem + Smem::kStats) + (uint32_t)slot * 8u, to);
+            const bool sends = i < ntok * G, some = ntiles > (halves ? x : 0);
+            if (sends) asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(stats), "f"(mref), "f"(l) : "memory");
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t w[32];
+                if (some) {
+                    tc::tmem_ld_x32(o_cols + (uint32_t)c, w);
+                    tc::tmem_ld_wait();
+                } else {
 #pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) {
-                const int k = min(k0 + e * NX * 128, mine * (HD / 4) - 1), i = rank + k / (HD / 4) * ns;
-                stats[e] = tc::smem_addr(smem + Smem::kStats + i * 8);              // (tile b's rows lie behind tile a's)
-                sums[e] = tc::smem_addr(smem + Smem::kSums) + (uint32_t)(i * T8_PITCH + k % (HD / 4) * 4) * 4u;
-                M[e] = -INFINITY;
-                L[e] = 0.f;
-                O[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            for (int z2 = 0; z2 < (halves ? 2 * ns : ns); ++z2) {
-                const uint32_t z = (uint32_t)(halves ? z2 >> 1 : z2), half = (uint32_t)(halves ? z2 & 1 : 0);
-                float m[kAtOnce], l[kAtOnce];
-                float4 o[kAtOnce];
-#pragma unroll
-                for (int e = 0; e < kAtOnce; ++e) {
-                    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[e]), "=f"(l[e]) : "r"(tc::map_to_rank(stats[e] + half * (BQ * 8), z)));
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                 : "=f"(o[e].x), "=f"(o[e].y), "=f"(o[e].z), "=f"(o[e].w) : "r"(tc::map_to_rank(sums[e] + half * (BQ * T8_PITCH * 4), z)));
+                    for (int d = 0; d < 32; ++d) w[d] = 0u;
                 }
 #pragma unroll
-                for (int e = 0; e < kAtOnce; ++e) {
-                    const float m_new = fmaxf(M[e], m[e]), use = m_new == -INFINITY ? 0.f : m_new;
-                    const float f = t8_exp2(M[e] - use), fz = t8_exp2(m[e] - use);
-                    M[e] = m_new;
-                    L[e] = L[e] * f + l[e] * fz;
-                    O[e].x = O[e].x * f + o[e].x * fz; O[e].y = O[e].y * f + o[e].y * fz;
-                    O[e].z = O[e].z * f + o[e].z * fz; O[e].w = O[e].w * f + o[e].w * fz;
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < kAtOnce; ++e) {
-                const int k = k0 + e * NX * 128, i = rank + k / (HD / 4) * ns, tok = i / G, hq = i - tok * G;
-                if (k >= mine * (HD / 4)) continue;
-                const float inv = L[e] == 0.f ? 0.f : 1.f / L[e];
-                uint2 v;
-                __nv_bfloat162* v2 = reinterpret_cast<__nv_bfloat162*>(&v);
-                v2[0] = __floats2bfloat162_rn(O[e].x * inv, O[e].y * inv);
-                v2[1] = __floats2bfloat162_rn(O[e].z * inv, O[e].w * inv);
-                *reinterpret_cast<uint2*>(p.out + ((size_t)(row0 + tok) * p.nh + head0 + hq) * HD + k % (HD / 4) * 4) = v;
+                for (int d = 0; d < 32; d += 4)
+                    if (sends)
+                        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sums + (uint32_t)(c + d) * 4u), "r"(w[d]),
+                                     "r"(w[d + 1]), "r"(w[d + 2]), "r"(w[d + 3])
+                                     : "memory");
             }
         }
-        tc::cluster_sync();                                // nobody leaves while its sums may be read
+        tc::cluster_sync();
+        const int mine = (ntok * G - rank + ns - 1) >> shift;
+        float2* all_stats = reinterpret_cast<float2*>(smem + Smem::kStats);
+        if ((int)threadIdx.x < mine) {
+            float2* stat = all_stats + threadIdx.x;
+            float M = -INFINITY, L = 0.f;
+#pragma unroll 1
+            for (int z = 0; z < sources; ++z) M = fmaxf(M, stat[z * rows].x);
+            const float use = M == -INFINITY ? 0.f : M;
+#pragma unroll 1
+            for (int z = 0; z < sources; ++z) L += stat[z * rows].y * t8_exp2(stat[z * rows].x - use);
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll 1
+            for (int z = 0; z < sources; ++z) stat[z * rows].x = t8_exp2(stat[z * rows].x - use) * inv;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int k = threadIdx.x; k < mine * (HD / 4); k += T8_THREADS(NX)) {
+            const int n = k / (HD / 4), d = k % (HD / 4) * 4;
+            const float* v = reinterpret_cast<const float*>(smem + Smem::kSums) + (size_t)n * T8_PITCH + d;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int z = 0; z < sources; ++z) {
+                const float w = all_stats[z * rows + n].x;
+                const float4 o = *reinterpret_cast<const float4*>(v + (size_t)z * rows * T8_PITCH);
+                acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y);
+                acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
+            }
+            const int i = (n << shift) + rank, tok = i / G, hq = i - tok * G;
+            uint2 u;
+            __nv_bfloat162* u2 = reinterpret_cast<__nv_bfloat162*>(&u);
+            u2[0] = __floats2bfloat162_rn(acc.x, acc.y);
+            u2[1] = __floats2bfloat162_rn(acc.z, acc.w);
+            *reinterpret_cast<uint2*>(p.out + ((size_t)(row0 + tok) * p.nh + head0 + hq) * HD + d) = u;
+        }
     }
     tc::fence_before_sync();
     __syncthreads();

@@ -195,12 +195,13 @@ def plan_portions(query_lens: Sequence[int], per_tile: int, num_kv_heads: int, k
     """(query tiles to a CTA, CTAs to a KV head, key slices) of the kernel for portions: query tiles of ``per_tile`` tokens, rows that see
     some ``keys`` keys on average.
 
-    Measured (one B200, 32 heads on 8 KV heads of 128, us).  Two query tiles share every key tile, and a CTA with only one of them
-    filled is no slower alone on its SM (2048 rows behind nothing: 58, one tile 68; 17 behind 8191: 37.7, one tile 38.4); but two CTAs of
-    one tile fit an SM, so one tile is taken where CTAs outnumber the SMs and a tenth of the second tiles would lie empty (32 sequences of
-    2 rows and 2000 keys: 125, two tiles 138; twelve prompts of 21 to 515 on heads of 64: 32.6, two tiles 35.8).  The keys are cut
-    while CTAs are fewer than SMs and a slice keeps some two tiles of 128 keys (512 rows behind 4096 keys: 61 in two, 90 whole; behind
-    nothing: 27 in two, 24 whole; 17 behind 1000: 20.5 in four, 21.6 in eight; 12 sequences of 32 rows and 1000 keys: 60 in two, 44 whole)."""
+    Measured (one B200, 32 heads on 8 KV heads of 128, us).  Two query tiles share every key tile, and where only one of them is filled
+    a CTA alone on its SM walks two key tiles at once (2048 rows behind nothing: 58, one tile 67; 17 behind 8191: 31, one tile 35); but
+    two CTAs of one tile fit an SM, so one tile is taken where CTAs outnumber the SMs and a tenth of the second tiles would lie empty
+    (32 sequences of 2 rows and 2000 keys: 123, two tiles 136; twelve prompts of 21 to 515 on heads of 64: 31, two tiles 35).  The
+    keys are cut while CTAs are fewer than SMs and a slice keeps some two tiles of 128 keys (512 rows behind 4096 keys: 59 in two,
+    88 whole; behind nothing: 24 in two, 22 whole; 64 behind 32000: 112 in eight, 170 in four; 12 sequences of 32 rows and 1000 keys: 54 in
+    two, 42 whole)."""
     single = sum(-(-n // per_tile) for n in query_lens)
     ctas = sum(-(-n // (2 * per_tile)) for n in query_lens)
     if ctas * num_kv_heads > sms and 10 * single <= 19 * ctas:
