@@ -876,6 +876,46 @@ AP_EXPORT int ap_attention_kv8_decode_takes(int P) { return (P == 8 || P == 16 |
 // Query heads of a product's columns: a KV head's, up to eight.
 static int k8d_heads(int nh, int nkv) { const int g = nh / nkv; return g < 8 ? g : 8; }
 
+// The attributes of the kernels, once on every device
+static int k8d_configure() {
+    static bool configured[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return AP_ERR_LAUNCH;
+    if (configured[dev]) return AP_OK;
+    const void* kernels[4] = {(const void*)attention_kv8_decode_kernel<1, false>, (const void*)attention_kv8_decode_kernel<2, false>,
+                              (const void*)attention_kv8_decode_kernel<1, true>, (const void*)attention_kv8_decode_kernel<2, true>};
+    for (int i = 0; i < 4; ++i) {
+        const int n = 1 + (i & 1);
+        if (cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 k8d_stages(n) * (STAGE_BYTES + SCALE_BYTES) + k8d_merge_bytes(n) + 1024) != cudaSuccess ||
+            (i >= 2 && cudaFuncSetAttribute(kernels[i], cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess))
+            return AP_ERR_LAUNCH;
+    }
+    configured[dev] = true;
+    return AP_OK;
+}
+
+// Clusters of `cluster` CTAs that the current device runs at a time (its SMs come in groups that a cluster does not straddle).
+AP_EXPORT int ap_attention_kv8_decode_clusters(int nh, int nkv, int cluster) {
+    if (cluster < 1 || cluster > 16 || nkv <= 0 || k8d_configure() != AP_OK) return 0;
+    const int nt = k8d_heads(nh, nkv) > 4 ? 2 : 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster, 1);
+    cfg.blockDim = dim3(K8D_THREADS);
+    cfg.dynamicSmemBytes = k8d_stages(nt) * (STAGE_BYTES + SCALE_BYTES) + k8d_merge_bytes(nt) + 1024;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const cudaError_t e = nt == 1 ? cudaOccupancyMaxActiveClusters(&n, attention_kv8_decode_kernel<1, true>, &cfg)
+                                  : cudaOccupancyMaxActiveClusters(&n, attention_kv8_decode_kernel<2, true>, &cfg);
+    if (e != cudaSuccess) cudaGetLastError();                  // (nothing to the next launch)
+    return e == cudaSuccess ? n : 0;
+}
+
 // Bytes of scratch that ap_attention_kv8_decode needs for `ctas` CTAs.
 AP_EXPORT long long ap_attention_kv8_decode_scratch(int nh, int nkv, int ctas) {
     return 16LL * ctas + 8LL * ctas * k8d_heads(nh, nkv) * XROW;
@@ -919,22 +959,7 @@ AP_EXPORT int ap_attention_kv8_decode(const void* q, void* out, const void* cach
     const int nt = heads > 4 ? 2 : 1;
     p.stages = k8d_stages(nt);
     const int smem = p.stages * (STAGE_BYTES + SCALE_BYTES) + k8d_merge_bytes(nt) + 1024;
-    static bool configured[64];
-    int dev = 0;
-    AP_REQUIRE(cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64, "attention_kv8: cannot tell the current device");
-    if (!configured[dev]) {
-        const void* kernels[4] = {(const void*)attention_kv8_decode_kernel<1, false>, (const void*)attention_kv8_decode_kernel<2, false>,
-                                  (const void*)attention_kv8_decode_kernel<1, true>, (const void*)attention_kv8_decode_kernel<2, true>};
-        cudaError_t e = cudaSuccess;
-        for (int i = 0; i < 4 && e == cudaSuccess; ++i) {
-            const int n = 1 + (i & 1);
-            e = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     k8d_stages(n) * (STAGE_BYTES + SCALE_BYTES) + k8d_merge_bytes(n) + 1024);
-            if (e == cudaSuccess && i >= 2) e = cudaFuncSetAttribute(kernels[i], cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        }
-        AP_REQUIRE(e == cudaSuccess, "attention_kv8: cannot configure the kernel: %s", cudaGetErrorString(e));
-        configured[dev] = true;
-    }
+    AP_REQUIRE(k8d_configure() == AP_OK, "attention_kv8: cannot configure the kernel for single rows");
     CUtensorMap map;
     {
         // [page][keys, values][KV head and row][number]: a box is a page of one head, its keys and its values

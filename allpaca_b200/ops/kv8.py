@@ -133,18 +133,26 @@ def _sms(device: int) -> int:
     return torch.cuda.get_device_properties(device).multi_processor_count
 
 
+@functools.lru_cache(maxsize=None)
+def _clusters(device: int, num_heads: int, num_kv_heads: int, head_dim: int):
+    """((CTAs to a cluster, such clusters that run at a time), ...) of the kernel for single rows."""
+    fits = library.attention(head_dim).ap_attention_kv8_decode_clusters
+    return tuple((c, fits(num_heads, num_kv_heads, c)) for c in (1, 2, 4, 8, 16))
+
+
 @functools.lru_cache(maxsize=4096)
-def plan_rows(pairs: int, longest: int, mean: int, sms: int):
+def plan_rows(pairs: int, longest: int, mean: int, sms: int, clusters):
     """(CTAs, CTAs to a cluster) of the kernel for single rows: ``pairs`` of a row and a KV head, of up to ``longest`` tiles of 64 keys,
-    ``mean`` on average.  Clusters (0: none) give every pair CTAs of its own.
+    ``mean`` on average; ``clusters`` as from :func:`_clusters`.  Clusters (0: none) give every pair CTAs of its own.
 
     Measured (one B200, pages scattered, us; a tile takes a CTA some 0.38 once its loads run): shared work costs 11 beside its tiles where
     pairs outnumber the CTAs (64 rows of 2048 keys on 8 KV heads: 54.6, in clusters of one 69.9), 16 where every pair is cut (8 rows of
-    4096: 27.5; clusters of two 20.7, of four 29.0).  A pair to a cluster costs 5.5, and 1.2 for putting parts together (1 row of 4096:
-    clusters of eight 10.3, shared 18.2; of 300: of one 6.2, shared 10.5), but a CTA to an SM it leaves SMs idle (1 row of
-    32768: shared 27.6, of eight 30.6), and the longest row sets its time."""
+    4096: 28.1; clusters of two 20.7).  A pair to a cluster costs 5.5, and 1.2 for putting parts together (1 row of 4096 keys: clusters
+    of eight 9.9, shared 13.9; on one KV head of sixteen 8.5, of eight 9.7), but a CTA to an SM it leaves SMs idle (1 row of 32768: shared
+    25.7, of eight 30.5), the longest row sets its time, and what does not fit at once takes a second turn (2 rows of 4096: of
+    eight 20.1, of four 13.0; the 148 SMs hold 15 of eight, 33 of four)."""
     best = ((16.0 if pairs < sms else 11.0) + 0.39 * pairs * mean / sms, max(1, min(sms, pairs * mean // 2)), 0)
-    for cluster, most in ((1, sms), (2, 64), (4, 32), (8, 16)):
+    for cluster, most in clusters:
         if pairs <= most and (cluster == 1 or longest >= cluster):
             best = min(best, (5.5 + 0.38 * -(-longest // cluster) + (1.2 if cluster > 1 else 0.0), pairs * cluster, cluster))
     return best[1:]
@@ -170,7 +178,8 @@ def _rows(q, out, cache, table, token_seq, positions, rows, num_heads, num_kv_he
     x, y, seq, pos, width = q.data_ptr(), out.data_ptr(), token_seq.data_ptr(), positions.data_ptr(), num_heads * head_dim
     for r in range(0, rows, step):
         n = min(step, rows - r)
-        ctas, cluster = plan_rows(n * sets, -(-longest // 64), -(-mean // 64), _sms(device))
+        ctas, cluster = plan_rows(n * sets, -(-longest // 64), -(-mean // 64), _sms(device),
+                                  _clusters(device, num_heads, num_kv_heads, head_dim))
         at, need = 0, 0
         if not cluster:
             need = _scratch_bytes(num_heads, num_kv_heads, head_dim, ctas)

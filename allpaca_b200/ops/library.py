@@ -249,6 +249,7 @@ _OPTIONAL_ATTN_SIGNATURES: Dict[str, list] = {
     "ap_attention_kv8_decode": [_P, _P, _P, _L, _L, _P, _I, _I, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _P, _L, _L, _P],
     "ap_attention_kv8_decode_scratch": [_I, _I, _I],
     "ap_attention_kv8_decode_takes": [_I],
+    "ap_attention_kv8_decode_clusters": [_I, _I, _I],
     "ap_attention_kv8_decode_status": [],
     # int ap_attention_kv8_tcgen05(q, out, cache, num_pages, page_bytes, block_table, max_blocks, seq_start, positions, nseq, T, nh, nkv, hd,
     #                              P, scale, window, query_tiles, total_ctas, nsplit, scratch, scratch_bytes, stream)
