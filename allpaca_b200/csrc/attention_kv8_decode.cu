@@ -3,11 +3,18 @@
 //
 // Such rows stream the cache; the rest has to stay out of the way.  One CTA to an SM lives through the whole launch: two warps
 // bring tiles of 64 keys (a TMA box to a page, the scale bytes by cp.async) into a ring in shared memory, eight warps work on
-// them, 32 keys at a time each.  The work, all tiles of all (row, KV head) pairs end to end, is
-// cut into equal runs, one to a CTA, so no SM waits for another whatever the lengths; the loads never pause, as the ring runs on from one
-// pair into the next, and two more warps prepare the next pair's queries and add up the last one's sums meanwhile.  (Loading with cp.async, any page size and no swizzle, took four warps 1500 to 2500 cycles of dependent
-// instructions to a tile: 2.5 TB/s.)  A pair that a cut falls into is put together by the CTA that finishes its part last: parts go to scratch,
-// nobody waits, and they are added in an order of their own.
+// them, 32 keys at a time each.  The work, all tiles of all (row, KV head) pairs end to end, is cut into runs of equal cost, one
+// to a CTA, so no SM waits for another whatever the lengths; the loads never pause, as the ring runs on from one pair into the next,
+// and two more warps prepare the next pair's queries and add up the last one's sums meanwhile.  (Loading with cp.async, any page size
+// and no swizzle, took four warps 1500 to 2500 cycles of dependent instructions to a tile: 2.5 TB/s.)  A pair that a cut falls
+// into is put together by the CTA that finishes its part last: parts go to scratch, nobody waits, and they are added in an order of
+// their own.  Few pairs get a cluster of CTAs each instead, whose parts meet in distributed shared memory.
+//
+// Bound by memory while it streams, at 5.8 to 6.4 TB/s with pages scattered: 64 rows of 2048 keys (8 KV heads of 128: 270 MB, floor 41.9 us at
+// the copy rate) take 54.6 us, of which 5.5 pass before the first tile is there (positions, block table and tile are read one after
+// the other) and 3 after the last.  One row of 32768 keys (floor 10.5) takes 25.7: 5.5, 10.5 of streaming, 9 until parts are written, seen
+// and added up.  Ragged rows (64 of 150 to 4096 keys, floor 24.7) take 47.8: each pair costs four tiles' time beside its own.  Heads of
+// 64 (64 rows of 4096 keys: 71, floor 42.2) are bound by what the working warps do per tile, which does not shrink with the head.
 //
 // The numbers are never widened: the products are e4m3 x e4m3 (mma.sync m16n8k32) with the keys, and the columns of the values, as
 // the 16 rows, and it is the queries and the weights that are split into two e4m3 numbers, x = hi + lo / 16, side by side in the

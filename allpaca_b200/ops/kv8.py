@@ -16,6 +16,9 @@ import torch
 
 from . import AP_BF16, AP_F32, KernelError, call, core, library, stream_handle
 
+# (a CUDA tensor is there before it is asked: nothing is left to initialise)
+_here = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
 _CODES = {torch.float32: AP_F32, torch.bfloat16: AP_BF16}
 
 
@@ -42,7 +45,7 @@ def _take_cache(what: str, cache_layer: torch.Tensor, num_kv_heads: int, head_di
         raise KernelError(f"{what}: {num_kv_heads} KV heads of {head_dim} in pages of {page_size} are not taken (head sizes are "
                           f"multiples of 16 up to 256)")
     device = cache_layer.get_device()
-    if device < 0 or device != torch.cuda.current_device():
+    if device < 0 or device != _here():
         raise KernelError(f"{what}: the cache must be a CUDA tensor on the current device, is on {cache_layer.device}")
     pages, page_bytes = _take(what, cache_layer, "cache_layer", torch.uint8, 2, device)
     cache = cache_layer.data_ptr()

@@ -296,7 +296,8 @@ def stream_handle() -> int:
         import torch
         fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         if fast is not None:
-            _raw_stream = lambda: fast(torch.cuda.current_device())          # noqa: E731
+            here = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+            _raw_stream = lambda: fast(here())                               # noqa: E731
         else:
             _raw_stream = lambda: torch.cuda.current_stream().cuda_stream    # noqa: E731
     return _raw_stream()
