@@ -144,21 +144,27 @@ def _clusters(device: int, num_heads: int, num_kv_heads: int, head_dim: int):
 
 
 @functools.lru_cache(maxsize=4096)
-def plan_rows(pairs: int, longest: int, mean: int, sms: int, clusters):
-    """(CTAs, CTAs to a cluster) of the kernel for single rows: ``pairs`` of a row and a KV head, of up to ``longest`` tiles of 64 keys,
+def _rows_cost(pairs: int, longest: int, mean: int, sms: int, clusters):
+    """(us, CTAs, CTAs to a cluster) of the kernel for single rows: ``pairs`` of a row and a KV head, of up to ``longest`` tiles of 64 keys,
     ``mean`` on average; ``clusters`` as from :func:`_clusters`.  Clusters (0: none) give every pair CTAs of its own.
 
-    Measured (one B200, pages scattered, us; a tile takes a CTA some 0.38 once its loads run): shared work costs 11 beside its tiles where
-    pairs outnumber the CTAs (64 rows of 2048 keys on 8 KV heads: 54.6, in clusters of one 69.9), 16 where every pair is cut (8 rows of
+    Measured (one B200, pages scattered, us; a tile takes a CTA some 0.38 once its loads run): shared work costs 6 and five tiles' time for
+    each pair beside its tiles where the CTAs hold several (64 rows of 2048 keys on 8 KV heads: 54.6, in clusters of one 69.9; 100 rows
+    of a prompt: 21.3), 16 where nearly every pair is cut (20 rows of 2000 keys: 31; 8 rows of
     4096: 28.1; clusters of two 20.7).  A pair to a cluster costs 5.5, and 1.2 for putting parts together (1 row of 4096 keys: clusters
     of eight 9.9, shared 13.9; on one KV head of sixteen 8.5, of eight 9.7), but a CTA to an SM it leaves SMs idle (1 row of 32768: shared
     25.7, of eight 30.5), the longest row sets its time, and what does not fit at once takes a second turn (2 rows of 4096: of
     eight 20.1, of four 13.0; the 148 SMs hold 15 of eight, 33 of four)."""
-    best = ((16.0 if pairs < sms else 11.0) + 0.39 * pairs * mean / sms, max(1, min(sms, pairs * mean // 2)), 0)
+    best = (16.0 + 0.39 * pairs * mean / sms if pairs < 2 * sms else 6.0 + 0.39 * pairs * (mean + 5) / sms, max(1, min(sms, pairs * mean // 2)), 0)
     for cluster, most in clusters:
         if pairs <= most and (cluster == 1 or longest >= cluster):
             best = min(best, (5.5 + 0.38 * -(-longest // cluster) + (1.2 if cluster > 1 else 0.0), pairs * cluster, cluster))
-    return best[1:]
+    return best
+
+
+def plan_rows(*work):
+    """(CTAs, CTAs to a cluster) for :func:`_rows_cost`'s work."""
+    return _rows_cost(*work)[1:]
 
 
 @functools.lru_cache(maxsize=None)
@@ -224,8 +230,33 @@ def plan_portions(query_lens: Sequence[int], per_tile: int, num_kv_heads: int, k
     return 2, ctas, slices
 
 
+@functools.lru_cache(maxsize=4096)
+def rows_are_faster(rows_us: float, sequences: int, longest: int, numbers: int, query_tiles: int, at_once: int, waves: int) -> bool:
+    """Whether portions are better taken row by row, which costs ``rows_us``.  The kernel for portions costs its start and end, the
+    widening of ``longest`` keys of ``numbers`` numbers to a sequence, and rounds of a key tile each.
+
+    Measured (one B200, 32 heads on 8 KV heads of 128, us; row by row, as portions): 17 rows behind 1000 keys 11.2, 16.8; behind 4000 28.2,
+    22.9; 64 rows behind 300 29.0, 17.5; 2 rows behind 30000 33.0, 69.3; 32 sequences of 2 rows and 2000 keys 54.5, 121; of 8 rows and 500
+    keys (64 sequences) 120, 72; 12 of 32 rows and 1000 keys 148, 40."""
+    rounds = -(-(-(-longest // 128)) // at_once)
+    return rows_us < 14.0 + 1e-6 * sequences * longest * numbers + (2.0 if query_tiles == 2 else 2.5) * rounds * waves
+
+
 # bytes of scratch for widened keys and values up to which sequences go together
 WIDE_SCRATCH = 1 << 30
+
+
+def _row_by_row(query_lens, per_tile, num_heads, num_kv_heads, head_dim, window, longest, device) -> bool:
+    """Whether the portions of ``query_lens`` go to the kernel for single rows."""
+    if window:
+        longest = min(longest, window + max(query_lens))
+    sms, sets = _sms(device), num_kv_heads * -(-(num_heads // num_kv_heads) // 8)
+    rows_us = _rows_cost(sum(query_lens) * sets, -(-longest // 64), -(-longest // 64), sms,
+                         _clusters(device, num_heads, num_kv_heads, head_dim))[0]
+    query_tiles, ctas, slices = plan_portions(query_lens, per_tile, num_kv_heads, longest - max(query_lens) // 2, sms)
+    at_once = slices * (2 if slices > 1 and max(query_lens) <= per_tile else 1)
+    return rows_are_faster(rows_us, len(query_lens), longest, num_kv_heads * head_dim, query_tiles, at_once,
+                           -(-ctas * num_kv_heads * slices // (sms * (3 - query_tiles))))
 
 
 def _portions(q, out, cache, table, seq_start, positions, first_seq, query_lens, T, num_heads, num_kv_heads, head_dim, page_size, scale,
@@ -282,7 +313,8 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
                 ones += 1
             if ones < len(query_lens):
                 per_tile = _portions_taken(num_heads, num_kv_heads, head_dim, page_size) if scale > 0 else 0
-                if per_tile:
+                if per_tile and not (T <= 512 and _row_by_row(query_lens[ones:], per_tile, num_heads, num_kv_heads, head_dim, window,
+                                                              max_context if max_context and not ones else widest, device)):
                     _portions(q, out, cache, table, seq_start, positions, ones, query_lens[ones:], T, num_heads, num_kv_heads, head_dim,
                               page_size, scale, window, per_tile, max_context if max_context and not ones else widest, scratch, device)
                     rows = ones

@@ -22,6 +22,14 @@ def ops():
     return o
 
 
+@pytest.fixture(params=["by rule", "tensor cores"])
+def portions(request, monkeypatch):
+    """Portions by the kernel that the rule names, then all by the one for portions, however small."""
+    from allpaca_b200.ops import kv8
+    if request.param == "tensor cores":
+        monkeypatch.setattr(kv8, "rows_are_faster", lambda *a: False)
+
+
 def dev(t):
     return t.to("cuda") if t is not None else None
 
@@ -157,6 +165,7 @@ def check(got, c, scale, window=0):
     assert float(worst) <= 1.0, float(worst)
 
 
+@pytest.mark.usefixtures("portions")
 @pytest.mark.parametrize("nh,nkv,hd,P", SHAPES)
 @pytest.mark.parametrize("seqs", [DECODE, MIXED], ids=["decode", "mixed"])
 @pytest.mark.parametrize("window", [0, 37, 200])
@@ -166,6 +175,7 @@ def test_attention(ops, nh, nkv, hd, P, seqs, window, dtype, metadata):
     check(run(ops, c, 0.8 / math.sqrt(hd), window, metadata), c, 0.8 / math.sqrt(hd), window)
 
 
+@pytest.mark.usefixtures("portions")
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("spread", [4.0, 12.0])
 @pytest.mark.parametrize("seqs", [DECODE, [(700, 300), (65, 65)]], ids=["decode", "portions"])
@@ -178,6 +188,7 @@ def test_attention_over_rows_of_unequal_size(ops, dtype, spread, seqs):
         check(run(ops, c, 1.0 / math.sqrt(hd)), c, 1.0 / math.sqrt(hd))
 
 
+@pytest.mark.usefixtures("portions")
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("far", [0, 3, 15, 16, 31, 32, 63, 64, 127, 128, 500, 1023])
 def test_finds_one_far_key(ops, dtype, far):
@@ -201,6 +212,7 @@ def test_finds_one_far_key(ops, dtype, far):
             assert float(((got - want).abs() / off).max()) <= 1.0
 
 
+@pytest.mark.usefixtures("portions")
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("seqs", [[(900, 1), (500, 1), (149, 1)], [(900, 70), (500, 3), (300, 149)]], ids=["decode", "portions"])
 def test_pages_given_back(ops, dtype, seqs):
@@ -284,6 +296,7 @@ def test_portions_on_tensor_cores(ops, query_tiles, slices, nh, nkv, hd, P, wind
     from allpaca_b200.ops import kv8
     monkeypatch.setattr(kv8, "plan_portions", lambda lens, per_tile, *a: (
         query_tiles, sum(-(-n // (query_tiles * per_tile)) for n in lens), slices))
+    monkeypatch.setattr(kv8, "rows_are_faster", lambda *a: False)
     monkeypatch.setattr(kv8, "WIDE_SCRATCH", (1 << 30) if slices < 4 else 1)          # all sequences together, or one by one
     for seqs in ([(1500, 2), (700, 70), (129, 129), (1, 1), (64, 1), (2, 2), (3000, 300)], [(130, 130)], [(257, 2)]):
         c = plain.case(seqs, nh, nkv, hd, P, torch.bfloat16, seed=slices + hd)

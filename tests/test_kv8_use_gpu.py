@@ -5,9 +5,9 @@ import pytest
 import torch
 
 import plain_kv8 as plain
-from test_kv8_gpu import DECODE, WEIGHTS, check, dev, ops, run   # noqa: F401
+from test_kv8_gpu import DECODE, WEIGHTS, dev, ops, portions, run   # noqa: F401
 
-pytestmark = pytest.mark.gpu
+pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("portions")]
 
 
 def rows_of(seqs):
