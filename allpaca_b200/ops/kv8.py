@@ -284,7 +284,7 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
                   query_lens: Optional[Sequence[int]] = None, max_context: int = 0, scratch=None,
                   mean_context: int = 0) -> None:
     """Causal attention of every row of ``q [T, nh*hd]`` over its sequence's keys in the 8-bit cache; arguments as for
-    :func:`attention`, with ``page_size`` beside the flat pages.  Scores, softmax and sums are 32-bit.  A row sees the keys at and
+    :func:`attention`, with ``page_size`` beside the flat pages (``max_context`` and ``mean_context`` only say how to cut the work).  Scores, softmax and sums are 32-bit.  A row sees the keys at and
     before its position (the last ``window`` of them, 0: all) whose page is there; one that sees none gets zeros.  The rows of a
     sequence follow one another and so do their positions."""
     what = "attention_kv8"
@@ -319,7 +319,7 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
                               page_size, scale, window, per_tile, max_context if max_context and not ones else widest, scratch, device)
                     rows = ones
         if rows:
-            longest = max_context if max_context and rows == ones else widest
+            longest = max_context if max_context and ones in (0, rows) else widest
             _rows(q, out, cache, table, token_seq, positions, rows, num_heads, num_kv_heads, head_dim, page_size, scale, window,
                   longest, min(mean_context or longest, longest), scratch, device)
         return

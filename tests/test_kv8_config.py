@@ -6,7 +6,7 @@ import plain_kv8
 from allpaca_b200 import ops
 from allpaca_b200.config import EngineConfig
 from allpaca_b200.config.model_config import ConfigError
-from allpaca_b200.parts import BuildEnv, KV8Need, KVNeed, Workspace, build, PartSpec
+from allpaca_b200.parts import BuildEnv, KV8Need, KVNeed, PartError, Workspace, build, PartSpec
 
 
 def test_settings():
@@ -40,6 +40,30 @@ def test_the_mixer_asks_for_it():
         env = BuildEnv(torch.float32, torch.device("cpu"), Workspace(torch.device("cpu")), kv_dtype=kv)
         need = build("mixer", spec, env).cache_need()
         assert isinstance(need, KV8Need) is kind and need.window == 32
+
+
+def test_head_sizes_that_no_kernel_takes():
+    env = BuildEnv(torch.float32, torch.device("cpu"), Workspace(torch.device("cpu")), kv_dtype="fp8")
+    for hd in (24, 272):
+        with pytest.raises(PartError):
+            build("mixer", PartSpec("gqa_attention", {"hidden_size": 64, "num_heads": 4, "num_kv_heads": 2, "head_dim": hd}), env)
+
+
+def test_plans():
+    """Work is cut into no more pieces than there are, and every sequence's rows find a CTA."""
+    from allpaca_b200.ops import kv8
+    fits = ((1, 148), (2, 74), (4, 33), (8, 15), (16, 7))
+    for pairs in (1, 7, 8, 15, 16, 33, 74, 148, 149, 512, 4096):
+        for longest in (1, 2, 5, 64, 1000):
+            for mean in {1, max(1, longest // 3), longest}:
+                ctas, cluster = kv8.plan_rows(pairs, longest, mean, 148, fits)
+                assert 1 <= ctas and (ctas <= 148 if cluster == 0 else ctas == pairs * cluster and pairs <= dict(fits)[cluster])
+    for lens in ([2], [1, 1, 5], [0, 7], [2048], [17] * 40, [600, 3], [31, 32, 33, 64, 65]):
+        for per_tile in (1, 8, 32, 128):
+            for keys in (0, 100, 5000, 100000):
+                tiles, ctas, slices = kv8.plan_portions(lens, per_tile, 8, keys, 148)
+                assert tiles in (1, 2) and slices in (1, 2, 4, 8) and ctas == sum(-(-n // (tiles * per_tile)) for n in lens)
+                assert slices == 1 or ctas * 8 * slices <= 148
 
 
 def test_no_cpu_branch():
