@@ -47,33 +47,33 @@ __device__ __forceinline__ uint32_t kv8_round4(const float4 x, float f) {
     return kv8_pack4(fmaf(x.x, f, x.x - x.x), fmaf(x.y, f, x.y - x.y), fmaf(x.z, f, x.z - x.z), fmaf(x.w, f, x.w - x.w));
 }
 
-// LPH lanes side by side take a head of a row (hd / 8 of them work): a lane holds numbers i .. i + 3 and i + hd/2 .. i + hd/2 + 3,
-// i = 4 * lane, which are four whole pairs of the rotation; the maximum goes round the lanes in registers, so the row is read
-// and written once.  The products of the rotation are rounded one by one (no fused multiply-add), so that the same inputs give the
-// same bytes as the formula computed step by step.
+// A CTA takes 256 lanes' worth of a row's heads, 2^side_bits lanes side by side a head, hd / 8 of which work: a lane holds numbers
+// i .. i + 3 and i + hd/2 .. i + hd/2 + 3, i four times its place, which are four whole pairs of the rotation; the maximum goes round
+// the lanes in registers, so the row is read and written once.  The products of the rotation are rounded one by one (no fused
+// multiply-add), so that the same inputs give the same bytes as the formula computed step by step.
 //
 // Few rows are bound by their launch and three loads that wait for one another (position, page, store): 1 row of a small model 2.5 us,
-// 64 rows 2.1 in a stream of such launches.  Many rows are bound by the time a warp is alive, from its first load to its last store: 2048
-// rows of 32 + 16 heads of 128 (47 MB, floor 7.3 us) take 14.3 us, 8192 rows 50.2.  Eight numbers to a half and lane, rows of
-// a prompt in turns of CTAs of 128 threads, were 13.3 and 42.6, but 64 rows 3.1; several heads to a thread with all loads ahead
-// were slower everywhere (two 19.4 for 2048 rows, four 29.9), and so was looking the page up ahead of the rotation (16.1).
-template <typename TI, typename TO, int LPH>
+// 64 rows 2.0 in a stream of such launches.  Many rows are bound by instructions (2.9 of 4 issued a cycle with a division for the
+// row and the pairing decided in the kernel; without them 2048 rows of 32 + 16 heads of 128, 47 MB, floor 7.3 us, take 12.7 us instead of
+// 14.3, 8192 rows 45.8 instead of 50.2).  Eight numbers to a half and lane, rows of a prompt in turns of CTAs of 128
+// threads, were 13.3 and 42.6, but 64 rows 3.1; several heads to a thread with all loads ahead were slower everywhere (two 19.4 for 2048
+// rows, four 29.9), and so was looking the page up ahead of the rotation (16.1).
+template <typename TI, typename TO, int PAIRING>
 __global__ void __launch_bounds__(KV8_THREADS, 6)
 rope_kv8_store_kernel(const TI* __restrict__ in, int S, size_t in_stride, TO* __restrict__ q_out, uint8_t* __restrict__ cache,
                       const int* __restrict__ positions, const int* __restrict__ token_seq, const int* __restrict__ block_table,
-                      int max_blocks, int nseq, const float2* __restrict__ cos_sin, int pairing, int T, int nh, int nkv, int hd, int P,
+                      int max_blocks, int nseq, const float2* __restrict__ cos_sin, int nh, int nkv, int hd, int P, int side_bits,
                       size_t page_bytes, int num_pages) {
-    const int heads = nh + 2 * nkv, lane = threadIdx.x & (LPH - 1), half = hd >> 1, i = lane * 4;
-    const unsigned id = blockIdx.x * (KV8_THREADS / LPH) + threadIdx.x / LPH;      // (fewer than 2^31: the launch checks)
-    const int t = (int)(id / (unsigned)heads), head = (int)(id - (unsigned)t * (unsigned)heads);
+    const int heads = nh + 2 * nkv, t = blockIdx.x, half = hd >> 1;
+    const int head = (blockIdx.y * KV8_THREADS + threadIdx.x) >> side_bits, i = (threadIdx.x & ((1 << side_bits) - 1)) * 4;
     ap_pdl_trigger();
     ap_pdl_wait();
-    const bool works = t < T && i < half, turns = head < nh + nkv;
+    const bool works = head < heads && i < half, turns = head < nh + nkv;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
     int at_a = i, at_b = i + half;                            // where the results go
     if (works) {
-        const TI* src = in + (size_t)id * hd;
-        const bool pairs = turns && pairing != 0;
+        const TI* src = in + (size_t)t * heads * hd + head * hd;
+        const bool pairs = PAIRING != 0 && turns;
         a = kv8_load4<TI>(src + (pairs ? 2 * i : i), S, in_stride);
         b = kv8_load4<TI>(src + (pairs ? 2 * i + 4 : i + half), S, in_stride);
         if (pairs) {
@@ -89,7 +89,7 @@ rope_kv8_store_kernel(const TI* __restrict__ in, int S, size_t in_stride, TO* __
             b = make_float4(__fadd_rn(__fmul_rn(x.x, c.y), __fmul_rn(b.x, c.x)), __fadd_rn(__fmul_rn(x.y, c.w), __fmul_rn(b.y, c.z)),
                             __fadd_rn(__fmul_rn(x.z, d.y), __fmul_rn(b.z, d.x)), __fadd_rn(__fmul_rn(x.w, d.w), __fmul_rn(b.w, d.z)));
         }
-        if (turns && pairing == 1) {                          // the results are neighbours as well
+        if (PAIRING == 1 && turns) {                          // the results are neighbours as well
             const float4 x = a;
             a = make_float4(x.x, b.x, x.y, b.y);
             b = make_float4(x.z, b.z, x.w, b.w);
@@ -97,7 +97,7 @@ rope_kv8_store_kernel(const TI* __restrict__ in, int S, size_t in_stride, TO* __
             at_b = 2 * i + 4;
         }
         if (head < nh) {
-            TO* dst = q_out + ((size_t)t * nh + head) * hd;
+            TO* dst = q_out + (size_t)t * nh * hd + head * hd;
             kv8_store4(dst + at_a, a);
             kv8_store4(dst + at_b, b);
         }
@@ -106,20 +106,21 @@ rope_kv8_store_kernel(const TI* __restrict__ in, int S, size_t in_stride, TO* __
     const bool kept = works && head >= nh;
     if (!__any_sync(0xffffffffu, kept)) return;
     uint32_t amax = kv8_largest(kv8_largest(0u, a), b);
-#pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int o = (1 << side_bits) >> 1; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (!kept) return;
     const int pos = positions[t], seq = token_seq[t];
-    if (pos < 0 || pos / P >= max_blocks || seq < 0 || seq >= nseq) return;
-    const int page = block_table[(size_t)seq * max_blocks + pos / P];
+    if (pos < 0 || seq < 0 || seq >= nseq) return;
+    const int block = pos / P;
+    if (block >= max_blocks) return;
+    const int page = block_table[(size_t)seq * max_blocks + block];
     if (page < 0 || page >= num_pages) return;                // a row without a page is not kept
     const int byte = kv8_scale_byte(amax);
     const float inv = __uint_as_float((uint32_t)(254 - byte) << 23);     // 2^-e
-    const size_t row = (size_t)(head - nh) * P + pos % P;
+    const size_t row = (size_t)(head - nh) * P + (pos - block * P);
     uint8_t* base = cache + (size_t)page * page_bytes;
     *reinterpret_cast<uint32_t*>(base + row * hd + at_a) = kv8_round4(a, inv);
     *reinterpret_cast<uint32_t*>(base + row * hd + at_b) = kv8_round4(b, inv);
-    if (lane == 0) base[(size_t)2 * nkv * P * hd + row] = (uint8_t)byte;
+    if (i == 0) base[(size_t)2 * nkv * P * hd + row] = (uint8_t)byte;
 }
 
 static int kv8_check(const char* what, const void* cache, long long num_pages, long long page_bytes, int nkv, int hd, int P,
@@ -146,27 +147,24 @@ AP_EXPORT int ap_rope_kv8_store(const void* in, int in_dtype, int S, long long i
     AP_REQUIRE(in_dtype == AP_F32 || S == 1, "rope_kv8_store: partial sums must be 32-bit");
     if (T == 0) return AP_OK;
     const int heads = nh + 2 * nkv, lanes = hd / 8;
-    const int lph = lanes <= 2 ? 2 : lanes <= 4 ? 4 : lanes <= 8 ? 8 : lanes <= 16 ? 16 : 32;
-    const int per = KV8_THREADS / lph;
-    AP_REQUIRE((long long)T * heads < (1LL << 31) - per, "rope_kv8_store: %d rows of %d heads exceed the grid", T, heads);
-    const unsigned ctas = (unsigned)(((long long)T * heads + per - 1) / per);
-#define KV8_STORE(TI, TO, L)                                                                                                        \
-    AP_CHECK_PDL_LAUNCH("rope_kv8_store", ap_launch_pdl(rope_kv8_store_kernel<TI, TO, L>, dim3(ctas), dim3(KV8_THREADS), 0, stream,  \
+    const int bits = lanes <= 2 ? 1 : lanes <= 4 ? 2 : lanes <= 8 ? 3 : lanes <= 16 ? 4 : 5;
+    AP_REQUIRE(heads <= (65535 * KV8_THREADS >> bits), "rope_kv8_store: %d heads exceed the grid", heads);
+    const dim3 grid((unsigned)T, (unsigned)(((heads << bits) + KV8_THREADS - 1) / KV8_THREADS));
+#define KV8_STORE(TI, TO, PAIRING)                                                                                                 \
+    AP_CHECK_PDL_LAUNCH("rope_kv8_store", ap_launch_pdl(rope_kv8_store_kernel<TI, TO, PAIRING>, grid, dim3(KV8_THREADS), 0, stream,  \
                         (const TI*)in, S, (size_t)in_stride, (TO*)q_out, (uint8_t*)cache, positions, token_seq, block_table, max_blocks, \
-                        nseq, (const float2*)cos_sin, pairing, T, nh, nkv, hd, P, (size_t)page_bytes, (int)num_pages))
-#define KV8_STORE_BY_LANES(TI, TO)                  \
+                        nseq, (const float2*)cos_sin, nh, nkv, hd, P, bits, (size_t)page_bytes, (int)num_pages))
+#define KV8_STORE_BY_PAIRING(TI, TO)                \
     do {                                            \
-        if (lph == 2) KV8_STORE(TI, TO, 2);         \
-        else if (lph == 4) KV8_STORE(TI, TO, 4);    \
-        else if (lph == 8) KV8_STORE(TI, TO, 8);    \
-        else if (lph == 16) KV8_STORE(TI, TO, 16);  \
-        else KV8_STORE(TI, TO, 32);                 \
+        if (pairing == 0) KV8_STORE(TI, TO, 0);     \
+        else if (pairing == 1) KV8_STORE(TI, TO, 1); \
+        else KV8_STORE(TI, TO, 2);                  \
     } while (0)
-    if (in_dtype == AP_F32 && act_dtype == AP_F32) KV8_STORE_BY_LANES(float, float);
-    else if (in_dtype == AP_F32 && act_dtype == AP_BF16) KV8_STORE_BY_LANES(float, bf16);
-    else if (in_dtype == AP_BF16 && act_dtype == AP_BF16) KV8_STORE_BY_LANES(bf16, bf16);
+    if (in_dtype == AP_F32 && act_dtype == AP_F32) KV8_STORE_BY_PAIRING(float, float);
+    else if (in_dtype == AP_F32 && act_dtype == AP_BF16) KV8_STORE_BY_PAIRING(float, bf16);
+    else if (in_dtype == AP_BF16 && act_dtype == AP_BF16) KV8_STORE_BY_PAIRING(bf16, bf16);
     else AP_REQUIRE(false, "rope_kv8_store: unsupported dtypes in=%d act=%d", in_dtype, act_dtype);
-#undef KV8_STORE_BY_LANES
+#undef KV8_STORE_BY_PAIRING
 #undef KV8_STORE
     return AP_OK;
 }
