@@ -137,16 +137,18 @@ def _sms(device: int) -> int:
 
 
 @functools.lru_cache(maxsize=None)
-def _clusters(device: int, num_heads: int, num_kv_heads: int, head_dim: int):
-    """((CTAs to a cluster, such clusters that run at a time), ...) of the kernel for single rows."""
-    fits = library.attention(head_dim).ap_attention_kv8_decode_clusters
-    return tuple((c, fits(num_heads, num_kv_heads, c)) for c in (1, 2, 4, 8, 16))
+def _machine(device: int, num_heads: int, num_kv_heads: int, head_dim: int):
+    """What the kernel for single rows runs on: its library, the SMs, ((CTAs to a cluster, such clusters that run at a time), ...), and the
+    pairs that a row makes (a KV head and up to eight of its query heads each)."""
+    lib = library.attention(head_dim)
+    clusters = tuple((c, lib.ap_attention_kv8_decode_clusters(num_heads, num_kv_heads, c)) for c in (1, 2, 4, 8, 16))
+    return lib, _sms(device), clusters, num_kv_heads * -(-(num_heads // num_kv_heads) // 8)
 
 
 @functools.lru_cache(maxsize=4096)
 def _rows_cost(pairs: int, longest: int, mean: int, sms: int, clusters):
     """(us, CTAs, CTAs to a cluster) of the kernel for single rows: ``pairs`` of a row and a KV head, of up to ``longest`` tiles of 64 keys,
-    ``mean`` on average; ``clusters`` as from :func:`_clusters`.  Clusters (0: none) give every pair CTAs of its own.
+    ``mean`` on average; ``clusters`` as from :func:`_machine`.  Clusters (0: none) give every pair CTAs of its own.
 
     Measured (one B200, pages scattered, us; a tile takes a CTA some 0.38 once its loads run): shared work costs 6 and five tiles' time for
     each pair beside its tiles where the CTAs hold several (64 rows of 2048 keys on 8 KV heads: 54.6, in clusters of one 69.9; 100 rows
@@ -180,24 +182,24 @@ def _scratch_bytes(num_heads: int, num_kv_heads: int, head_dim: int, ctas: int) 
 def _rows(q, out, cache, table, token_seq, positions, rows, num_heads, num_kv_heads, head_dim, page_size, scale, window, longest, mean,
           scratch, device) -> None:
     """The first ``rows`` rows one by one, up to ``longest`` keys to a row and some ``mean``."""
-    lib = library.attention(head_dim)
+    lib, sms, clusters, sets = _machine(device, num_heads, num_kv_heads, head_dim)
     if window:
         longest, mean = min(longest, window + 64), min(mean, window + 64)
-    step, sets = 512, num_kv_heads * -(-(num_heads // num_kv_heads) // 8)
+    step = 512
     x, y, seq, pos, width = q.data_ptr(), out.data_ptr(), token_seq.data_ptr(), positions.data_ptr(), num_heads * head_dim
     for r in range(0, rows, step):
         n = min(step, rows - r)
-        ctas, cluster = plan_rows(n * sets, -(-longest // 64), -(-mean // 64), _sms(device),
-                                  _clusters(device, num_heads, num_kv_heads, head_dim))
-        at, need = 0, 0
+        ctas, cluster = plan_rows(n * sets, -(-longest // 64), -(-mean // 64), sms, clusters)
+        at, need, nonce = 0, 0, 0
         if not cluster:
+            nonce = next(_nonces) % (1 << 62) + 1
             need = _scratch_bytes(num_heads, num_kv_heads, head_dim, ctas)
             buf = scratch("attn.kv8", (need // 4,), torch.float32) if scratch is not None else \
                 torch.empty(need // 4, dtype=torch.float32, device=q.device)
             at = buf.data_ptr()
         call(lib, "ap_attention_kv8_decode", x + 2 * r * width, y + 2 * r * width, *cache, *table, seq + 4 * r, pos + 4 * r, n,
              num_heads, num_kv_heads, head_dim, page_size, float(scale), int(window), ctas, cluster, at, need,
-             next(_nonces) % (1 << 62) + 1, stream_handle())
+             nonce, stream_handle())
 
 
 @functools.lru_cache(maxsize=None)
@@ -250,9 +252,8 @@ def _row_by_row(query_lens, per_tile, num_heads, num_kv_heads, head_dim, window,
     """Whether the portions of ``query_lens`` go to the kernel for single rows."""
     if window:
         longest = min(longest, window + max(query_lens))
-    sms, sets = _sms(device), num_kv_heads * -(-(num_heads // num_kv_heads) // 8)
-    rows_us = _rows_cost(sum(query_lens) * sets, -(-longest // 64), -(-longest // 64), sms,
-                         _clusters(device, num_heads, num_kv_heads, head_dim))[0]
+    _, sms, clusters, sets = _machine(device, num_heads, num_kv_heads, head_dim)
+    rows_us = _rows_cost(sum(query_lens) * sets, -(-longest // 64), -(-longest // 64), sms, clusters)[0]
     query_tiles, ctas, slices = plan_portions(query_lens, per_tile, num_kv_heads, longest - max(query_lens) // 2, sms)
     at_once = slices * (2 if slices > 1 and max(query_lens) <= per_tile else 1)
     return rows_are_faster(rows_us, len(query_lens), longest, num_kv_heads * head_dim, query_tiles, at_once,
@@ -309,8 +310,8 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
         widest = table[1] * page_size
         ones, rows = 0, T
         if by_sequence:
-            while ones < len(query_lens) and query_lens[ones] == 1:
-                ones += 1
+            # (as many sequences as rows: one each, or none and several here and there, which the rows' own metadata says as well)
+            ones = next((i for i, n in enumerate(query_lens) if n != 1), len(query_lens)) if len(query_lens) != T else T
             if ones < len(query_lens):
                 per_tile = _portions_taken(num_heads, num_kv_heads, head_dim, page_size) if scale > 0 else 0
                 if per_tile and not (T <= 512 and _row_by_row(query_lens[ones:], per_tile, num_heads, num_kv_heads, head_dim, window,

@@ -249,3 +249,11 @@ def test_long_tables(ops):   # noqa: F811
         case["table"] = narrow
         want, off = plain.attend(case, 0.1, 0, WEIGHTS)
         assert float(((got - want).abs() / off).max()) <= 1.0
+
+
+@pytest.mark.parametrize("seqs", [[(50, 0), (90, 2)], [(90, 2), (40, 0), (70, 1)], [(64, 1), (30, 0), (200, 70)], [(30, 0), (70, 1), (65, 1)]])
+def test_sequences_that_bring_nothing(ops, seqs):   # noqa: F811
+    for dtype in (torch.bfloat16, torch.float32):
+        c = plain.case(seqs, 8, 2, 64, 16, dtype, seed=10)
+        want, off = plain.attend(c, 0.1, 0, WEIGHTS if dtype == torch.bfloat16 else 0.0)
+        assert float(((run(ops, c, 0.1) - want).abs() / off).max()) <= 1.0
