@@ -288,7 +288,8 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
     __shared__ int s_last[K8D_MAX_ROWS], s_seq[K8D_MAX_ROWS];   // the last key a row sees (-1: none) and its sequence
     __shared__ int s_warp[K8D_THREADS / 32];
     __shared__ int s_dead, s_join[2];
-    __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], q_full[2], q_empty[2], dumped, taken, join;
+    __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES], q_full[2], q_empty[2], dumped, taken;
+    __shared__ uint64_t join[2];                           // of either late pair: one is decided while a warp may still wait for the other
     __shared__ uint32_t s_query[2][NT][CHUNKS + 1][32];    // a pair's queries as the products take them; last: the rows' factors
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* scales = smem + (size_t)p.stages * STAGE_BYTES;
@@ -302,10 +303,10 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&q_full[i], 1);
             tc::mbar_init(&q_empty[i], CWARPS);
+            tc::mbar_init(&join[i], 1);
         }
         tc::mbar_init(&dumped, CWARPS);
         tc::mbar_init(&taken, 1);
-        tc::mbar_init(&join, 1);
         tc::fence_barrier_init();
         tc::prefetch_tensormap(&tmap);
         s_dead = *(volatile int*)&g_k8d_status;            // one reading for all, as they meet at barriers
@@ -605,7 +606,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
             const bool all = all_there(late[i].item0, late[i].nparts);
             if (lane == 0) s_join[i] = all ? 1 : 0;
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&join);
+            if (lane == 0) tc::mbar_arrive(&join[i]);
             if (!all) continue;
             if (!__all_sync(0xffffffffu, tc::mbar_wait(&dumped, ph))) {
                 give_up();
@@ -813,7 +814,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
     }
     // pairs of many parts: where all are there, bring them, this warp every CWARPS-th
     for (int i = 0; i < n_late; ++i) {
-        if (!ok || !__all_sync(0xffffffffu, tc::mbar_wait(&join, (uint32_t)(i & 1)))) {
+        if (!ok || !__all_sync(0xffffffffu, tc::mbar_wait(&join[i], 0))) {
             give_up();
             return;
         }
