@@ -2,7 +2,8 @@
 // 64 and 128 (-DAP_HEAD_DIM): sequences that bring several new rows each, from two on, packed one behind the other.
 //
 // Two kernels.  The first widens the keys that the step's rows see, once: c * 2^e, exact in bfloat16, from pages into dense rows of
-// scratch memory, a sequence's keys of one KV head one behind the other; what lies outside, or has no page, becomes zeros.  The
+// scratch memory, a sequence's keys of one KV head one behind the other; what lies outside, or has no page, becomes zeros, and so do values
+// that are not finite (their NaN is put back at the end, in the rows that see them: looking for them costs 0 to 3 % of the call).  The
 // second has the arithmetic of attention_tcgen05_wide.cu: a CTA owns up to 256 rows, two tiles "a" and "b" of (128 / group) tokens x the
 // `group` query heads of one KV head, and every tile of 128 keys serves both; S and O live in tensor memory, the two tiles take turns
 // on the tensor cores while the other's softmax warps work (one row to a thread, P in bfloat16 over the S it came from, O scaled
@@ -68,6 +69,9 @@ __device__ __forceinline__ float t8_exp2(float x) {
 
 struct AttnT8Params {
     bf16* out;
+    const uint8_t* cache;
+    size_t page_bytes;
+    int* spoiled;                                         // [sequence][KV head][tile of its keys]: a value in it is not finite
     const int* block_table;
     const int* seq_start;
     const int* positions;
@@ -83,10 +87,17 @@ __device__ __forceinline__ void t8_span(const int* positions, int row0, int ntok
     kmin = (window > 0 && first - window + 1 > 0) ? first - window + 1 : 0;
 }
 
+// 0x80 in the bytes of a word of e4m3 numbers that are NaN
+__device__ __forceinline__ uint32_t t8_not_finite(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // ---- widening: grid (tiles of a sequence's keys, keys and values of every KV head, sequences) ----
+// Values that are not finite become zeros here, since the product with the values takes every row of a query tile at once and a weight of
+// zero does not undo a NaN; the tile is noted, and the rows that do see the value get their NaN at the second kernel's end.
 #define T8_WIDEN_THREADS 256
 __global__ void __launch_bounds__(T8_WIDEN_THREADS)
-kv8_widen_kernel(const uint8_t* __restrict__ cache, size_t page_bytes, const AttnT8Params p, bf16* __restrict__ dense) {
+kv8_widen_kernel(const __grid_constant__ AttnT8Params p, bf16* __restrict__ dense) {
+    const uint8_t* __restrict__ const cache = p.cache;
+    const size_t page_bytes = p.page_bytes;
     __shared__ long long at_s[BKV];                       // where a key's numbers lie (-1: nowhere)
     __shared__ float scale_s[BKV];
     const int s = blockIdx.z, plane = blockIdx.y, t = blockIdx.x;
@@ -123,6 +134,18 @@ kv8_widen_kernel(const uint8_t* __restrict__ cache, size_t page_bytes, const Att
         const int e = i * T8_WIDEN_THREADS + threadIdx.x, r = e / (HD / 8);
         const long long at = at_s[r];
         u[i] = at >= 0 ? *reinterpret_cast<const uint2*>(cache + at + (e - r * (HD / 8)) * 8) : make_uint2(0u, 0u);
+    }
+    if (plane >= p.nkv) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const uint32_t x = t8_not_finite(u[i].x), y = t8_not_finite(u[i].y);
+            u[i].x &= ~((x >> 7) * 0xffu);
+            u[i].y &= ~((y >> 7) * 0xffu);
+            bad |= x | y;
+        }
+        const int any = __syncthreads_or((int)bad);
+        if (threadIdx.x == 0) p.spoiled[((size_t)s * p.nkv + plane - p.nkv) * (p.cap / BKV) + t] = any ? 1 : 0;
     }
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
@@ -172,6 +195,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     volatile int* s_seq = (volatile int*)(tmem_slot + 2);
     volatile int* s_tile = (volatile int*)(tmem_slot + 3);
+    volatile int* s_spoiled = (volatile int*)(tmem_slot + 4);     // a value among the keys of the CTA's rows is not finite
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per_cta = NX * p.tokens_per_tile;           // tokens of one CTA
@@ -188,6 +212,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
             tc::mbar_init(&o_full[x], 1);
         }
         *abort_flag = 0;
+        *s_spoiled = 0;
         tc::fence_barrier_init();
         tc::prefetch_tensormap(&tmap_q);
         tc::prefetch_tensormap(&tmap_kv);
@@ -302,6 +327,15 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                     if (NX == 2 && fine) fine = load(it, v_row, v_full, v_free, Smem::kV);
                 }
             }
+        }
+    } else if (warp == kMmaWarp + 1) {
+        if (active) {
+            ap_pdl_wait();                                 // the widened keys and values
+            const int* flags = p.spoiled + ((size_t)seq * p.nkv + kvh) * (p.cap / BKV);
+            int bad = 0;
+            for (int t = kmin / BKV + lane; t <= kmax / BKV; t += 32) bad |= __ldcg(flags + t);
+            bad = __any_sync(0xffffffffu, bad != 0);
+            if (lane == 0) *s_spoiled = bad;
         }
     } else if (warp == kMmaWarp) {
         if (lane == 0 && active && ntiles > 0) {
@@ -614,6 +648,40 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     }
     tc::fence_before_sync();
     __syncthreads();
+    if (*s_spoiled && warp < kLoadWarp) {
+        // Rows that see a value which is not finite: its column becomes NaN.  A row to a lane, among those that this CTA wrote; the 32 lanes
+        // look at 32 keys at a time and tell one another which of them are spoiled, column by column.  (Whose rows they are is
+        // looked up again: the registers were the softmax's.)
+        const int s = *s_seq, first_row = p.seq_start[s] + *s_tile * per_cta, n = min(per_cta, p.seq_start[s + 1] - first_row);
+        const int head = (int)(blockIdx.x % (unsigned)p.nkv), i = (SPLIT ? p.nsplit : 1) * (int)threadIdx.x + (SPLIT ? (int)blockIdx.y : 0);
+        const bool row = i < n * p.group;
+        const int tok = row ? i / p.group : 0, last_key = p.max_blocks * p.P - 1;
+        const int pos = row ? min(p.positions[first_row + tok], last_key) : -1;
+        bf16* dst = p.out + ((size_t)(first_row + tok) * p.nh + head * p.group + (row ? i - tok * p.group : 0)) * HD;
+        const int* flags = p.spoiled + ((size_t)s * p.nkv + head) * (p.cap / BKV);
+        int k_first, k_last;
+        t8_span(p.positions, first_row, n, p.window, last_key, k_first, k_last);
+        for (int t = k_first / BKV; t <= k_last / BKV; ++t) {
+            if (__ldcg(flags + t) == 0) continue;
+            for (int k0 = t * BKV; k0 < (t + 1) * BKV; k0 += 32) {
+                const int key = k0 + lane;
+                const int page = key >= k_first && key <= k_last ? p.block_table[(size_t)s * p.max_blocks + key / p.P] : -1;
+                const bool there = page >= 0 && page < p.num_pages;
+                const uint8_t* v = p.cache + (there ? (size_t)page * p.page_bytes + ((size_t)(p.nkv + head) * p.P + key % p.P) * HD : 0);
+                // of these keys the row sees lo .. hi
+                const int lo = p.window > 0 ? max(pos - p.window + 1 - k0, 0) : 0, hi = min(pos - k0, 31);
+                const uint32_t sees = hi < lo ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+#pragma unroll 1
+                for (int w = 0; w < HD; w += 4) {
+                    const uint32_t bad = there ? t8_not_finite(*reinterpret_cast<const uint32_t*>(v + w)) : 0u;
+                    if (!__any_sync(0xffffffffu, bad != 0)) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (__ballot_sync(0xffffffffu, bad >> (8 * e) & 0x80u) & sees) dst[w + e] = __float2bfloat16(NAN);
+                }
+            }
+        }
+    }
     ap_pdl_trigger();
     if (warp == kMmaWarp) {
         __syncwarp();
@@ -651,7 +719,8 @@ AP_EXPORT int ap_attention_kv8_tcgen05_tokens(int nh, int nkv) { return 128 / (n
 
 // Bytes of scratch for `nseq` sequences with block tables of `max_blocks` pages
 AP_EXPORT long long ap_attention_kv8_tcgen05_scratch(int nseq, int max_blocks, int P, int nkv) {
-    return 2LL * nseq * 2 * nkv * (((long long)max_blocks * P + BKV - 1) / BKV * BKV) * HD;
+    const long long tiles = ((long long)max_blocks * P + BKV - 1) / BKV;
+    return (2LL * nseq * 2 * nkv * tiles * BKV * HD + 4LL * nseq * nkv * tiles + 15) / 16 * 16;
 }
 
 // q: [T][nh][HD]; query_tiles: 1 or 2 to a CTA; total_ctas: the sum over the sequences of ceil(rows / tokens of a CTA); nsplit: 1, 2, 4 or 8 key slices; scale > 0;
@@ -712,13 +781,13 @@ AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cac
         configured[dev] = true;
     }
     AttnT8Params p;
+    p.cache = (const uint8_t*)cache; p.page_bytes = (size_t)page_bytes; p.spoiled = (int*)((bf16*)scratch + (size_t)dense_rows * HD);
     p.out = (bf16*)out; p.block_table = block_table; p.seq_start = seq_start; p.positions = positions;
     p.cap = (int)cap; p.num_pages = (int)num_pages; p.max_blocks = max_blocks; p.nseq = nseq; p.nh = nh; p.nkv = nkv;
     p.P = P; p.window = window; p.group = G; p.tokens_per_tile = 128 / G; p.nsplit = nsplit;
     p.scale_log2 = scale * LOG2E_F;
     AP_REQUIRE((long long)total_ctas * nkv < (1LL << 31), "attention_kv8 (tcgen05): too many CTAs for the grid");
-    AP_CHECK_PDL_LAUNCH("kv8_widen", ap_launch_pdl(kv8_widen_kernel, dim3((unsigned)(cap / BKV), 2 * nkv, nseq), dim3(T8_WIDEN_THREADS), 0, stream,
-                                                     (const uint8_t*)cache, (size_t)page_bytes, p, (bf16*)scratch));
+    AP_CHECK_PDL_LAUNCH("kv8_widen", ap_launch_pdl(kv8_widen_kernel, dim3((unsigned)(cap / BKV), 2 * nkv, nseq), dim3(T8_WIDEN_THREADS), 0, stream, p, (bf16*)scratch));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(total_ctas * nkv), nsplit);
     cfg.blockDim = dim3(T8_THREADS(query_tiles));

@@ -287,7 +287,8 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
     """Causal attention of every row of ``q [T, nh*hd]`` over its sequence's keys in the 8-bit cache; arguments as for
     :func:`attention`, with ``page_size`` beside the flat pages (``max_context`` and ``mean_context`` only say how to cut the work).
     Scores, softmax and sums are 32-bit.  A row sees the keys at and before its position (the last ``window`` of them, 0: all) whose
-    page is there; one that sees none gets zeros.  The rows of a sequence follow one another and so do their positions; ``out`` is
+    page is there; one that sees none gets zeros.  A key that is not finite makes the rows that see it NaN, a value their columns of it, no
+    other row.  The rows of a sequence follow one another and so do their positions; ``out`` is
     another tensor than ``q``.  Calls that may run at the same time need scratch of their own (None: each allocates it)."""
     what = "attention_kv8"
     device, T, cache, table = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
