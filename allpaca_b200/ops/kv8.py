@@ -248,6 +248,19 @@ def rows_are_faster(rows_us: float, sequences: int, longest: int, numbers: int, 
 WIDE_SCRATCH = 1 << 30
 
 
+def step_lengths(query_lens: Sequence[int], ones: int, contexts: Optional[Sequence[int]], max_context: int, mean_context: int,
+                 widest: int):
+    """What a step with portions from sequence ``ones`` on is planned by: (longest context from there on, longest and average context of all
+    rows).  Where ``contexts`` does not say, ``max_context`` counts only if there are no one-row sequences that it may stand for,
+    else the width of the block table."""
+    if contexts is None:
+        longest = min(max_context if max_context and not ones and 1 not in query_lens else widest, widest)
+        return longest, longest, min(mean_context or longest, longest)
+    longest = min(max(contexts), widest)
+    mean = sum(c * n for c, n in zip(contexts, query_lens)) // max(1, sum(query_lens))
+    return max(1, min(max(contexts[ones:]), widest)), max(1, longest), max(1, min(mean, longest))
+
+
 def _row_by_row(query_lens, per_tile, num_heads, num_kv_heads, head_dim, window, longest, device) -> bool:
     """Whether the portions of ``query_lens`` go to the kernel for single rows."""
     if window:
@@ -283,10 +296,11 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
                   token_seq: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
                   page_size: int, scale: float, window: int = 0, seq_start: Optional[torch.Tensor] = None,
                   query_lens: Optional[Sequence[int]] = None, max_context: int = 0, scratch=None,
-                  mean_context: int = 0) -> None:
+                  mean_context: int = 0, contexts: Optional[Sequence[int]] = None) -> None:
     """Causal attention of every row of ``q [T, nh*hd]`` over its sequence's keys in the 8-bit cache; arguments as for
     :func:`attention`, with ``page_size`` beside the flat pages (``max_context`` and ``mean_context`` only say how to cut the work).
-    Scores, softmax and sums are 32-bit.  A row sees the keys at and before its position (the last ``window`` of them, 0: all) whose
+    ``contexts`` (host, one to a sequence of ``query_lens``): the sequences' keys, the newest row's among them; without it portions
+    are planned by ``max_context`` where no sequence brings one row, else by the width of the block table.  Scores, softmax and sums are 32-bit.  A row sees the keys at and before its position (the last ``window`` of them, 0: all) whose
     page is there; one that sees none gets zeros.  A key that is not finite makes the rows that see it NaN, a value their columns of it, no
     other row.  The rows of a sequence follow one another and so do their positions; ``out`` is
     another tensor than ``q``.  Calls that may run at the same time need scratch of their own (None: each allocates it)."""
@@ -305,26 +319,32 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
         starts, = _take(what, seq_start, "seq_start", torch.int32, 1, device)
         if starts != len(query_lens) + 1 or sum(query_lens) != T or table[2] < len(query_lens):
             raise KernelError(f"{what}: seq_start, query_lens and the block table do not describe the rows")
+    if contexts is not None and (not by_sequence or len(contexts) != len(query_lens)):
+        raise KernelError(f"{what}: contexts must name one number to a sequence of query_lens")
     if not T:
         return
     if code == AP_BF16 and 0 < cache[1] * cache[2] < 1 << 36 and _single_rows_taken(head_dim, page_size):
         # sequences that bring one row each, then portions (one-row sequences further back ride along with them)
         widest = table[1] * page_size
         ones, rows = 0, T
+        longest = min(max_context or widest, widest)
+        mean = min(mean_context or longest, longest)
         if by_sequence:
             # (as many sequences as rows: one each, or none and several here and there, which the rows' own metadata says as well)
             ones = next((i for i, n in enumerate(query_lens) if n != 1), len(query_lens)) if len(query_lens) != T else T
             if ones < len(query_lens):
+                behind, all_longest, all_mean = step_lengths(query_lens, ones, contexts, max_context, mean_context, widest)
                 per_tile = _portions_taken(num_heads, num_kv_heads, head_dim, page_size) if scale > 0 else 0
                 if per_tile and not (T <= 512 and _row_by_row(query_lens[ones:], per_tile, num_heads, num_kv_heads, head_dim, window,
-                                                              max_context if max_context and not ones else widest, device)):
+                                                              behind, device)):
                     _portions(q, out, cache, table, seq_start, positions, ones, query_lens[ones:], T, num_heads, num_kv_heads, head_dim,
-                              page_size, scale, window, per_tile, max_context if max_context and not ones else widest, scratch, device)
+                              page_size, scale, window, per_tile, behind, scratch, device)
                     rows = ones
+                else:
+                    longest, mean = all_longest, all_mean
         if rows:
-            longest = max_context if max_context and ones in (0, rows) else widest
             _rows(q, out, cache, table, token_seq, positions, rows, num_heads, num_kv_heads, head_dim, page_size, scale, window,
-                  longest, min(mean_context or longest, longest), scratch, device)
+                  longest, mean, scratch, device)
         return
     call(library.attention(head_dim), "ap_attention_kv8_rows", q.data_ptr(), out.data_ptr(), code, *cache, *table,
          token_seq.data_ptr(), positions.data_ptr(), T, num_heads, num_kv_heads, head_dim, page_size, float(scale), int(window),

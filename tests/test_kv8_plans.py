@@ -1,0 +1,127 @@
+"""What a step over the 8-bit cache is planned by, where there is no GPU: the entry points are recorded, not called."""
+import types
+
+import pytest
+import torch
+
+from allpaca_b200.ops import kv8
+
+HEADS = (32, 8, 128, 16)          # query heads, KV heads, head size, page size
+
+
+class Library:
+    """Stands in for the kernels' library on a device of 148 SMs."""
+    ap_attention_kv8_decode_takes = staticmethod(lambda P: 1)
+    ap_attention_kv8_decode_scratch = staticmethod(lambda nh, nkv, ctas: 1024)
+    ap_attention_kv8_decode_clusters = staticmethod(lambda nh, nkv, c: {1: 148, 2: 74, 4: 33, 8: 15, 16: 7}[c])
+    ap_attention_kv8_tcgen05_takes = staticmethod(lambda nh, nkv, hd, P: 1)
+    ap_attention_kv8_tcgen05_tokens = staticmethod(lambda nh, nkv: 128 // (nh // nkv))
+    ap_attention_kv8_tcgen05_scratch = staticmethod(lambda *a: 4096)
+
+
+@pytest.fixture
+def step(monkeypatch):
+    """step(seqs of (keys, rows), ...) -> [(entry point, how it is planned)]."""
+    caches = [kv8._machine, kv8._single_rows_taken, kv8._portions_taken, kv8._scratch_bytes]
+    for f in caches:
+        f.cache_clear()
+    calls, planned = [], []
+    rows_cost, plan_portions = kv8._rows_cost, kv8.plan_portions
+
+    def rows(pairs, longest, mean, *more):
+        planned.append((longest * 64, mean * 64))
+        return rows_cost(pairs, longest, mean, *more)
+
+    def portions(lens, per_tile, nkv, keys, sms):
+        planned.append((keys, plan_portions(lens, per_tile, nkv, keys, sms)))
+        return planned[-1][1]
+    monkeypatch.setattr(kv8, "library", types.SimpleNamespace(attention=lambda hd: Library))
+    monkeypatch.setattr(kv8, "_sms", lambda device: 148)
+    monkeypatch.setattr(kv8, "stream_handle", lambda: 0)
+    monkeypatch.setattr(kv8, "call", lambda lib, name, *a: calls.append((name, planned[-1])))
+    monkeypatch.setattr(kv8, "_rows_cost", rows)
+    monkeypatch.setattr(kv8, "plan_portions", portions)
+    monkeypatch.setattr(kv8, "_take_cache", lambda what, cache, nkv, hd, P, pos, seq, table: (
+        -1, seq.shape[0], (0, cache.shape[0], cache.shape[1]), (0, table.shape[1], table.shape[0])))
+
+    def run(seqs, **more):
+        nh, nkv, hd, P = HEADS
+        del calls[:], planned[:]
+        T, lens = sum(n for _, n in seqs), [n for _, n in seqs]
+        ints = lambda n: torch.zeros(n, dtype=torch.int32)   # noqa: E731
+        q = torch.zeros((T, nh * hd), dtype=torch.bfloat16)
+        table = torch.zeros((len(seqs), max(-(-c // P) for c, _ in seqs)), dtype=torch.int32)
+        kv8.attention_kv8(q, torch.zeros_like(q), torch.zeros((1, 16), dtype=torch.uint8), table, ints(T), ints(T), nh, nkv, hd, P, 0.1,
+                          seq_start=ints(len(seqs) + 1), query_lens=lens, **more)
+        return list(calls)
+    yield run
+    for f in caches:
+        f.cache_clear()
+
+
+PORTIONS, ROWS = "ap_attention_kv8_tcgen05", "ap_attention_kv8_decode"
+
+
+def contexts(seqs):
+    return [c for c, _ in seqs]
+
+
+def test_a_one_row_sequence_behind_a_portion(step):
+    """17 rows behind 30000 keys are far faster as portions; that the row behind them has ten keys changes nothing, whatever
+    the caller says of the longest one-row sequence."""
+    alone = step([(30017, 17)], max_context=30017)
+    assert alone[0][0] == PORTIONS and alone[0][1][1][2] == 8
+    seqs = [(30017, 17), (10, 1)]
+    for more in ({}, {"contexts": contexts(seqs)}):
+        (name, (keys, plan)), = step(seqs, max_context=10, mean_context=10, **more)
+        assert name == PORTIONS and keys > 29000 and plan[2] == 8
+    # more rows: their plan has key slices as well
+    (name, (keys, plan)), = step([(30512, 512), (10, 1)], max_context=10, mean_context=10, contexts=[30512, 10])
+    alone = step([(30512, 512)], max_context=30512)[0][1][1]
+    assert name == PORTIONS and keys > 29000 and alone[2] > 1 and plan == (alone[0], alone[1] + 1, alone[2])   # (one CTA for the row behind)
+
+
+def test_a_long_decoded_row_in_front_of_short_portions(step):
+    """One row of 131072 keys: the portions behind it are planned by their own keys, not by the block table's width."""
+    seqs = [(131072, 1), (317, 17)]
+    got = step(seqs, max_context=131072, mean_context=131072, contexts=contexts(seqs))
+    assert [name for name, _ in got] == [ROWS]                         # 17 rows behind 300 keys go row by row
+    longest, mean = got[0][1]
+    assert longest >= 131072 and mean < 8000                           # eighteen rows, one of them long
+    seqs = [(131072, 1), (512, 512), (400, 400)]
+    got = step(seqs, max_context=131072, mean_context=131072, contexts=contexts(seqs))
+    assert [name for name, _ in got] == [PORTIONS, ROWS]
+    assert got[0][1] == step(seqs[1:], max_context=512)[0][1]
+    assert got[1][1] == step(seqs[:1], max_context=131072)[0][1]
+
+
+def test_without_contexts(step):
+    """Portions alone are planned by max_context, or by the block table's width."""
+    assert step([(2512, 512)], max_context=2512) == step([(2512, 512)]) == step([(2512, 512)], contexts=[2512])
+    (_, (keys, _)), = step([(2512, 512), (90000, 600)], max_context=2512)
+    assert keys < 2512
+    (_, (keys, _)), = step([(2512, 512), (90000, 1)], max_context=2512)
+    assert keys > 80000
+
+
+def test_contexts_that_do_not_fit(step):
+    from allpaca_b200.ops import KernelError
+    with pytest.raises(KernelError):
+        step([(50, 2), (60, 1)], contexts=[50])
+
+
+def test_the_engine_says_how_long_its_sequences_are(monkeypatch):
+    """A step with portions names every sequence's keys; one of single rows leaves them out."""
+    from allpaca_b200.engine.batch import StepBatch
+    from allpaca_b200.parts import BuildEnv, LayerCache, PartSpec, Workspace, attention, build
+    seen = []
+    monkeypatch.setattr(attention.ops, "attention_kv8", lambda *a, **kw: seen.append(kw["contexts"]))
+    env = BuildEnv(torch.bfloat16, torch.device("cpu"), Workspace(torch.device("cpu")), kv_dtype="fp8")
+    mixer = build("mixer", PartSpec("gqa_attention", {"hidden_size": 64, "num_heads": 4, "num_kv_heads": 2, "head_dim": 16}), env)
+    for firsts, lens, want in (([40, 0, 7], [1, 30, 5], [41, 30, 12]), ([40, 8], [1, 1], None)):
+        T = sum(lens)
+        none = torch.zeros(T, dtype=torch.int32)
+        step = StepBatch(T, len(lens), 0, none, none, none, none, none, none, none, [none], host_first_position=firsts,
+                         host_query_lens=lens, max_query_len=max(lens))
+        mixer._attention(torch.zeros(T, 64, dtype=torch.bfloat16), T, step, LayerCache(group=0), env.workspace)
+        assert seen.pop() == want
