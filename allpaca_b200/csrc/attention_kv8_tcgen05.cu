@@ -76,15 +76,22 @@ struct AttnT8Params {
     const int* seq_start;
     const int* positions;
     int num_pages, max_blocks, nseq, nh, nkv, P, window, group, tokens_per_tile;   // tokens_per_tile: of one query tile
-    int nsplit, cap;                                      // cap: dense rows of a sequence's keys in one KV head, whole tiles
+    int nsplit, tiles;                                    // tiles: dense ones of a sequence's keys in one KV head
     float scale_log2;
 };
 
-// What the rows of sequence s see: tiles t_lo .. t_hi of its keys (none: t_hi < t_lo), keys kmin .. kmax
+// The keys kmin .. kmax that `ntok` rows from row0 on see (kmax < 0: none)
 __device__ __forceinline__ void t8_span(const int* positions, int row0, int ntok, int window, int last_key, int& kmin, int& kmax) {
     kmax = min(positions[row0 + ntok - 1], last_key);
     const int first = min(positions[row0], last_key);
     kmin = (window > 0 && first - window + 1 > 0) ? first - window + 1 : 0;
+}
+
+// A sequence's dense tiles hold its keys from tile t0 on, the first that its rows see, up to last_key
+__device__ __forceinline__ void t8_dense(const AttnT8Params& p, int first_row, int& t0, int& last_key) {
+    const int last = p.max_blocks * p.P - 1;
+    t0 = p.window > 0 ? max(min(p.positions[first_row], last) - p.window + 1, 0) / BKV : 0;
+    last_key = (int)min((long long)last, ((long long)t0 + p.tiles) * BKV - 1);
 }
 
 // 0x80 in the bytes of a word of e4m3 numbers that are NaN
@@ -100,15 +107,17 @@ kv8_widen_kernel(const __grid_constant__ AttnT8Params p, bf16* __restrict__ dens
     const size_t page_bytes = p.page_bytes;
     __shared__ long long at_s[BKV];                       // where a key's numbers lie (-1: nowhere)
     __shared__ float scale_s[BKV];
-    const int s = blockIdx.z, plane = blockIdx.y, t = blockIdx.x;
+    const int s = blockIdx.z, plane = blockIdx.y;
     // the second kernel may start once everything before this one has ended: it reads all but this one's result ahead of its own wait
     ap_pdl_wait();
     ap_pdl_trigger();
     const int row0 = p.seq_start[s], ntok = p.seq_start[s + 1] - row0;
     if (ntok <= 0) return;
-    int kmin, kmax;
-    t8_span(p.positions, row0, ntok, p.window, p.max_blocks * p.P - 1, kmin, kmax);
-    if (kmax < 0 ? t > 0 : (t < kmin / BKV || t > kmax / BKV)) return;      // (rows that see nothing still multiply one tile)
+    int kmin, kmax, t0, last_key;
+    t8_dense(p, row0, t0, last_key);
+    t8_span(p.positions, row0, ntok, p.window, last_key, kmin, kmax);
+    const int t = t0 + blockIdx.x;
+    if (kmax < 0 ? t > 0 : t > kmax / BKV) return;                          // (rows that see nothing still multiply one tile)
     if (threadIdx.x < BKV) {
         const int kpos = t * BKV + threadIdx.x;
         long long at = -1;
@@ -126,7 +135,7 @@ kv8_widen_kernel(const __grid_constant__ AttnT8Params p, bf16* __restrict__ dens
     }
     __syncthreads();
     // eight numbers to a thread and turn: whole rows of 8-byte loads and 16-byte stores side by side
-    bf16* to = dense + (((size_t)s * 2 * p.nkv + plane) * p.cap + (size_t)t * BKV) * HD;
+    bf16* to = dense + (((size_t)s * 2 * p.nkv + plane) * p.tiles + blockIdx.x) * BKV * HD;
     constexpr int kItems = BKV * HD / 8 / T8_WIDEN_THREADS;
     uint2 u[kItems];
 #pragma unroll
@@ -145,7 +154,7 @@ kv8_widen_kernel(const __grid_constant__ AttnT8Params p, bf16* __restrict__ dens
             bad |= x | y;
         }
         const int any = __syncthreads_or((int)bad);
-        if (threadIdx.x == 0) p.spoiled[((size_t)s * p.nkv + plane - p.nkv) * (p.cap / BKV) + t] = any ? 1 : 0;
+        if (threadIdx.x == 0) p.spoiled[((size_t)s * p.nkv + plane - p.nkv) * p.tiles + blockIdx.x] = any ? 1 : 0;
     }
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
@@ -256,7 +265,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
 
     // geometry of this CTA (identical in every thread)
     const int G = p.group;
-    int row0 = 0, ntok = 0, kmax = -1, kmin = 0, kvh = 0, head0 = 0;
+    int row0 = 0, ntok = 0, kmax = -1, kmin = 0, kvh = 0, head0 = 0, t0 = 0, last_key = -1;
     if (active) {
         row0 = p.seq_start[seq] + *s_tile * per_cta;
         ntok = min(per_cta, p.seq_start[seq + 1] - row0);
@@ -267,7 +276,9 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     // Where there is no second tile its place takes every other key tile of the first one's rows, as one more slice
     const bool halves = SPLIT && NX == 2 && !has_b;
     if (active) {
-        t8_span(p.positions, row0, ntok, p.window, p.max_blocks * p.P - 1, kmin, kmax);
+        t8_dense(p, p.seq_start[seq], t0, last_key);
+        t8_span(p.positions, row0, ntok, p.window, last_key, kmin, kmax);
+        kmin = max(kmin, t0 * BKV);                        // (positions that do not rise find no tile before the first)
     }
     int t_lo = kmin / BKV, t_hi = active ? kmax / BKV : -1;
     if (SPLIT) {
@@ -305,7 +316,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
                         tc::tma_load_3d(smem + Smem::kQ + x * Q_BYTES + h * SUB_BYTES, &tmap_q, h * 64, head0,
                                         row0 + x * p.tokens_per_tile, q_full);
                 ap_pdl_wait();                             // the widened keys and values
-                const int k_row = (seq * 2 * p.nkv + kvh) * p.cap + t_lo * BKV, v_row = k_row + p.nkv * p.cap;
+                const int k_row = ((seq * 2 * p.nkv + kvh) * p.tiles + t_lo - t0) * BKV, v_row = k_row + p.nkv * p.tiles * BKV;
                 auto load = [&](int it, int row, uint64_t* full, uint64_t* free, int base) -> bool {
                     const int s = it % kStages;
                     if (*abort_flag) return false;
@@ -331,7 +342,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
     } else if (warp == kMmaWarp + 1) {
         if (active) {
             ap_pdl_wait();                                 // the widened keys and values
-            const int* flags = p.spoiled + ((size_t)seq * p.nkv + kvh) * (p.cap / BKV);
+            const int* flags = p.spoiled + ((size_t)seq * p.nkv + kvh) * p.tiles - t0;
             int bad = 0;
             for (int t = kmin / BKV + lane; t <= kmax / BKV; t += 32) bad |= __ldcg(flags + t);
             bad = __any_sync(0xffffffffu, bad != 0);
@@ -439,7 +450,7 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         const uint32_t lane_base = tmem_base + ((uint32_t)(qtr * 32) << 16);
         const uint32_t s_cols = lane_base + (uint32_t)(x * BKV);
         const uint32_t o_cols = lane_base + (uint32_t)(kOCol + x * HD);
-        const int qpos = min(p.positions[row0 + (rvalid ? tok : 0)], p.max_blocks * p.P - 1);
+        const int qpos = min(p.positions[row0 + (rvalid ? tok : 0)], last_key);
         int page = page_of(it0);
         uint32_t ph = 0;
         for (int it = it0; it < ntiles; it += step, ph ^= 1u) {
@@ -655,13 +666,14 @@ attention_kv8_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_q, const _
         const int s = *s_seq, first_row = p.seq_start[s] + *s_tile * per_cta, n = min(per_cta, p.seq_start[s + 1] - first_row);
         const int head = (int)(blockIdx.x % (unsigned)p.nkv), i = (SPLIT ? p.nsplit : 1) * (int)threadIdx.x + (SPLIT ? (int)blockIdx.y : 0);
         const bool row = i < n * p.group;
-        const int tok = row ? i / p.group : 0, last_key = p.max_blocks * p.P - 1;
-        const int pos = row ? min(p.positions[first_row + tok], last_key) : -1;
+        const int tok = row ? i / p.group : 0;
+        int k_first, k_last, t_first, last;
+        t8_dense(p, p.seq_start[s], t_first, last);
+        t8_span(p.positions, first_row, n, p.window, last, k_first, k_last);
+        const int pos = row ? min(p.positions[first_row + tok], last) : -1;
         bf16* dst = p.out + ((size_t)(first_row + tok) * p.nh + head * p.group + (row ? i - tok * p.group : 0)) * HD;
-        const int* flags = p.spoiled + ((size_t)s * p.nkv + head) * (p.cap / BKV);
-        int k_first, k_last;
-        t8_span(p.positions, first_row, n, p.window, last_key, k_first, k_last);
-        for (int t = k_first / BKV; t <= k_last / BKV; ++t) {
+        const int* flags = p.spoiled + ((size_t)s * p.nkv + head) * p.tiles - t_first;
+        for (int t = max(k_first / BKV, t_first); t <= k_last / BKV; ++t) {
             if (__ldcg(flags + t) == 0) continue;
             for (int k0 = t * BKV; k0 < (t + 1) * BKV; k0 += 32) {
                 const int key = k0 + lane;
@@ -717,17 +729,17 @@ AP_EXPORT int ap_attention_kv8_tcgen05_takes(int nh, int nkv, int hd, int P) {
 // tokens of one sequence in a query tile
 AP_EXPORT int ap_attention_kv8_tcgen05_tokens(int nh, int nkv) { return 128 / (nh / nkv); }
 
-// Bytes of scratch for `nseq` sequences with block tables of `max_blocks` pages
-AP_EXPORT long long ap_attention_kv8_tcgen05_scratch(int nseq, int max_blocks, int P, int nkv) {
-    const long long tiles = ((long long)max_blocks * P + BKV - 1) / BKV;
-    return (2LL * nseq * 2 * nkv * tiles * BKV * HD + 4LL * nseq * nkv * tiles + 15) / 16 * 16;
+// Bytes of scratch for `tiles` tiles of 128 keys, of all sequences together
+AP_EXPORT long long ap_attention_kv8_tcgen05_scratch(long long tiles, int nkv) {
+    return (tiles * nkv * (2 * 2 * BKV * HD + 4) + 15) / 16 * 16;
 }
 
 // q: [T][nh][HD]; query_tiles: 1 or 2 to a CTA; total_ctas: the sum over the sequences of ceil(rows / tokens of a CTA); nsplit: 1, 2, 4 or 8 key slices; scale > 0;
-// scratch: ap_attention_kv8_tcgen05_scratch bytes of any contents, 16-byte aligned, of no call that runs at the same time.
+// tiles: tiles of 128 keys that a sequence's rows see at most, from the first one that they see on (keys beyond them are not seen);
+// scratch: ap_attention_kv8_tcgen05_scratch(nseq * tiles, nkv) bytes of any contents, 16-byte aligned, of no call that runs at the same time.
 AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cache, long long num_pages, long long page_bytes,
                                        const int* block_table, int max_blocks, const int* seq_start, const int* positions, int nseq, int T,
-                                       int nh, int nkv, int hd, int P, float scale, int window, int query_tiles, int total_ctas, int nsplit, void* scratch,
+                                       int nh, int nkv, int hd, int P, float scale, int window, int query_tiles, int total_ctas, int nsplit, int tiles, void* scratch,
                                        long long scratch_bytes, cudaStream_t stream) {
     AP_REQUIRE(ap_attention_kv8_tcgen05_takes(nh, nkv, hd, P), "attention_kv8 (tcgen05): shape not supported: heads=%d kv_heads=%d "
                "head_dim=%d page=%d", nh, nkv, hd, P);
@@ -735,9 +747,11 @@ AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cac
     AP_REQUIRE(num_pages >= 0 && num_pages < (1LL << 31) && page_bytes == kv8_page_bytes(nkv, P, HD), "attention_kv8: the pages do not match the heads");
     AP_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)cache & 15) == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)scratch & 15) == 0,
                "attention_kv8 (tcgen05): operands must be 16-byte aligned");
-    const long long cap = ((long long)max_blocks * P + BKV - 1) / BKV * BKV, dense_rows = (long long)nseq * 2 * nkv * cap;
+    AP_REQUIRE((long long)max_blocks * P < (1LL << 31) - 128, "attention_kv8 (tcgen05): the block table names more than 2^31 keys");
+    AP_REQUIRE(tiles > 0 && tiles < (1 << 24), "attention_kv8 (tcgen05): %d tiles of keys", tiles);
+    const long long dense_rows = (long long)nseq * 2 * nkv * tiles * BKV;
     AP_REQUIRE(dense_rows < (1LL << 31) - 256, "attention_kv8 (tcgen05): %lld rows of keys and values are too many", dense_rows);
-    AP_REQUIRE(scratch && scratch_bytes >= ap_attention_kv8_tcgen05_scratch(nseq, max_blocks, P, nkv), "attention_kv8 (tcgen05): %lld bytes of "
+    AP_REQUIRE(scratch && scratch_bytes >= ap_attention_kv8_tcgen05_scratch((long long)nseq * tiles, nkv), "attention_kv8 (tcgen05): %lld bytes of "
                "scratch are too few", scratch_bytes);
     AP_REQUIRE(query_tiles == 1 || query_tiles == 2, "attention_kv8 (tcgen05): %d query tiles", query_tiles);
     AP_REQUIRE(scale > 0.f, "attention_kv8 (tcgen05): the scale must be positive");
@@ -783,11 +797,11 @@ AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cac
     AttnT8Params p;
     p.cache = (const uint8_t*)cache; p.page_bytes = (size_t)page_bytes; p.spoiled = (int*)((bf16*)scratch + (size_t)dense_rows * HD);
     p.out = (bf16*)out; p.block_table = block_table; p.seq_start = seq_start; p.positions = positions;
-    p.cap = (int)cap; p.num_pages = (int)num_pages; p.max_blocks = max_blocks; p.nseq = nseq; p.nh = nh; p.nkv = nkv;
+    p.tiles = tiles; p.num_pages = (int)num_pages; p.max_blocks = max_blocks; p.nseq = nseq; p.nh = nh; p.nkv = nkv;
     p.P = P; p.window = window; p.group = G; p.tokens_per_tile = 128 / G; p.nsplit = nsplit;
     p.scale_log2 = scale * LOG2E_F;
     AP_REQUIRE((long long)total_ctas * nkv < (1LL << 31), "attention_kv8 (tcgen05): too many CTAs for the grid");
-    AP_CHECK_PDL_LAUNCH("kv8_widen", ap_launch_pdl(kv8_widen_kernel, dim3((unsigned)(cap / BKV), 2 * nkv, nseq), dim3(T8_WIDEN_THREADS), 0, stream, p, (bf16*)scratch));
+    AP_CHECK_PDL_LAUNCH("kv8_widen", ap_launch_pdl(kv8_widen_kernel, dim3((unsigned)tiles, 2 * nkv, nseq), dim3(T8_WIDEN_THREADS), 0, stream, p, (bf16*)scratch));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(total_ctas * nkv), nsplit);
     cfg.blockDim = dim3(T8_THREADS(query_tiles));

@@ -273,23 +273,45 @@ def _row_by_row(query_lens, per_tile, num_heads, num_kv_heads, head_dim, window,
                            -(-ctas * num_kv_heads * slices // (sms * (3 - query_tiles))))
 
 
+def dense_tiles(rows: int, keys: int, window: int) -> int:
+    """Tiles of 128 keys that a sequence of ``keys`` keys has among those that its last ``rows`` rows see."""
+    tiles = -(-keys // 128)
+    return max(1, min(tiles, (window + rows + 125) // 128 + 1) if window else tiles)      # (window + rows - 1 keys from anywhere on)
+
+
+def group_portions(query_lens: Sequence[int], contexts: Sequence[int], window: int, most: int):
+    """[(first sequence, one past the last, tiles of each), ...]: neighbours go together while their dense tiles, as many for each as the
+    longest needs, are no more than ``most``; one alone always goes."""
+    groups, first, widest = [], 0, 0
+    for i, (rows, keys) in enumerate(zip(query_lens, contexts)):
+        tiles = dense_tiles(rows, keys, window)
+        if i > first and max(widest, tiles) * (i + 1 - first) > most:
+            groups.append((first, i, widest))
+            first, widest = i, 0
+        widest = max(widest, tiles)
+    return groups + [(first, len(query_lens), widest)]
+
+
 def _portions(q, out, cache, table, seq_start, positions, first_seq, query_lens, T, num_heads, num_kv_heads, head_dim, page_size, scale,
-              window, per_tile, longest, scratch, device) -> None:
-    """The sequences from ``first_seq`` on, by their ``query_lens``, of up to ``longest`` keys; their rows follow those of the sequences
-    before."""
+              window, per_tile, longest, contexts, scratch, device) -> None:
+    """The sequences from ``first_seq`` on, by their ``query_lens``, of ``contexts`` keys each, or (None) some ``longest``; their rows follow
+    those of the sequences before."""
     (blocks, width, _), lib = table, library.attention(head_dim)
-    one = lib.ap_attention_kv8_tcgen05_scratch(1, width, page_size, num_kv_heads)
-    step = max(1, min(len(query_lens), WIDE_SCRATCH // one))
-    buf = scratch("attn.kv8_wide", (step * one // 2,), torch.bfloat16) if scratch is not None else \
-        torch.empty(step * one // 2, dtype=torch.bfloat16, device=q.device)
-    longest = min(longest, window + max(query_lens)) if window else longest
-    for at in range(0, len(query_lens), step):
-        lens = query_lens[at:at + step]
-        query_tiles, ctas, slices = plan_portions(lens, per_tile, num_kv_heads, longest - max(lens) // 2, _sms(device))
+    widest = width * page_size
+    keys = [widest] * len(query_lens) if contexts is None else [max(1, min(c, widest)) for c in contexts]
+    groups = group_portions(query_lens, keys, window, WIDE_SCRATCH // lib.ap_attention_kv8_tcgen05_scratch(1, num_kv_heads))
+    need = lib.ap_attention_kv8_tcgen05_scratch(max((end - at) * tiles for at, end, tiles in groups), num_kv_heads)
+    buf = scratch("attn.kv8_wide", (need // 2,), torch.bfloat16) if scratch is not None else \
+        torch.empty(need // 2, dtype=torch.bfloat16, device=q.device)
+    for at, end, tiles in groups:
+        lens, most = query_lens[at:end], longest if contexts is None else max(keys[at:end])
+        if window:
+            most = min(most, window + max(lens))
+        query_tiles, ctas, slices = plan_portions(lens, per_tile, num_kv_heads, most - max(lens) // 2, _sms(device))
         if ctas:
             call(lib, "ap_attention_kv8_tcgen05", q.data_ptr(), out.data_ptr(), *cache, blocks + 4 * (first_seq + at) * width, width,
                  seq_start.data_ptr() + 4 * (first_seq + at), positions.data_ptr(), len(lens), T, num_heads, num_kv_heads, head_dim,
-                 page_size, float(scale), int(window), query_tiles, ctas, slices, buf.data_ptr(), step * one, stream_handle())
+                 page_size, float(scale), int(window), query_tiles, ctas, slices, tiles, buf.data_ptr(), need, stream_handle())
 
 
 def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor, block_table: torch.Tensor,
@@ -299,8 +321,9 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
                   mean_context: int = 0, contexts: Optional[Sequence[int]] = None) -> None:
     """Causal attention of every row of ``q [T, nh*hd]`` over its sequence's keys in the 8-bit cache; arguments as for
     :func:`attention`, with ``page_size`` beside the flat pages (``max_context`` and ``mean_context`` only say how to cut the work).
-    ``contexts`` (host, one to a sequence of ``query_lens``): the sequences' keys, the newest row's among them; without it portions
-    are planned by ``max_context`` where no sequence brings one row, else by the width of the block table.  Scores, softmax and sums are 32-bit.  A row sees the keys at and before its position (the last ``window`` of them, 0: all) whose
+    ``contexts`` (host, one to a sequence of ``query_lens``): the sequences' keys, the newest row's among them (none may have
+    more); without it portions are planned by ``max_context`` where no sequence brings one row, else by the width of the block table, and their
+    scratch is as wide as the table.  Scores, softmax and sums are 32-bit.  A row sees the keys at and before its position (the last ``window`` of them, 0: all) whose
     page is there; one that sees none gets zeros.  A key that is not finite makes the rows that see it NaN, a value their columns of it, no
     other row.  The rows of a sequence follow one another and so do their positions; ``out`` is
     another tensor than ``q``.  Calls that may run at the same time need scratch of their own (None: each allocates it)."""
@@ -338,7 +361,7 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
                 if per_tile and not (T <= 512 and _row_by_row(query_lens[ones:], per_tile, num_heads, num_kv_heads, head_dim, window,
                                                               behind, device)):
                     _portions(q, out, cache, table, seq_start, positions, ones, query_lens[ones:], T, num_heads, num_kv_heads, head_dim,
-                              page_size, scale, window, per_tile, behind, scratch, device)
+                              page_size, scale, window, per_tile, behind, None if contexts is None else contexts[ones:], scratch, device)
                     rows = ones
                 else:
                     longest, mean = all_longest, all_mean

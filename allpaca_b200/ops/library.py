@@ -252,9 +252,9 @@ _OPTIONAL_ATTN_SIGNATURES: Dict[str, list] = {
     "ap_attention_kv8_decode_clusters": [_I, _I, _I],
     "ap_attention_kv8_decode_status": [],
     # int ap_attention_kv8_tcgen05(q, out, cache, num_pages, page_bytes, block_table, max_blocks, seq_start, positions, nseq, T, nh, nkv, hd,
-    #                              P, scale, window, query_tiles, total_ctas, nsplit, scratch, scratch_bytes, stream)
-    "ap_attention_kv8_tcgen05": [_P, _P, _P, _L, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P, _L, _P],
-    "ap_attention_kv8_tcgen05_scratch": [_I, _I, _I, _I],
+    #                              P, scale, window, query_tiles, total_ctas, nsplit, tiles, scratch, scratch_bytes, stream)
+    "ap_attention_kv8_tcgen05": [_P, _P, _P, _L, _L, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I, _I, _P, _L, _P],
+    "ap_attention_kv8_tcgen05_scratch": [_L, _I],
     "ap_attention_kv8_tcgen05_takes": [_I, _I, _I, _I],
     "ap_attention_kv8_tcgen05_tokens": [_I, _I],
     "ap_attention_kv8_tcgen05_status": [],

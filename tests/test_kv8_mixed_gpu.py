@@ -21,3 +21,12 @@ def test_with_and_without_contexts(ops, nh, nkv, hd, P, seqs, window, dtype):   
     for more in ({}, {"contexts": [k for k, _ in seqs]}, {"contexts": [k + 77 for k, _ in seqs]}):
         got = run(ops, c, 0.09, window, **more)
         assert float(((got - want).abs() / off).max()) <= 1.0
+
+
+def test_contexts_that_are_too_short_harm_no_other_sequence(ops):   # noqa: F811
+    seqs = [(2100, 300), (300, 300), (900, 120)]
+    for window in (0, 100):
+        c = plain.case(seqs, 8, 2, 128, 16, torch.bfloat16, seed=3)
+        want, off = plain.attend(c, 0.09, window, WEIGHTS)
+        got = run(ops, c, 0.09, window, contexts=[5, 300, 900])
+        assert float(((got - want).abs() / off)[300:].max()) <= 1.0

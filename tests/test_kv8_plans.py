@@ -16,7 +16,7 @@ class Library:
     ap_attention_kv8_decode_clusters = staticmethod(lambda nh, nkv, c: {1: 148, 2: 74, 4: 33, 8: 15, 16: 7}[c])
     ap_attention_kv8_tcgen05_takes = staticmethod(lambda nh, nkv, hd, P: 1)
     ap_attention_kv8_tcgen05_tokens = staticmethod(lambda nh, nkv: 128 // (nh // nkv))
-    ap_attention_kv8_tcgen05_scratch = staticmethod(lambda *a: 4096)
+    ap_attention_kv8_tcgen05_scratch = staticmethod(lambda tiles, nkv: tiles * nkv * (4 * 128 * HEADS[2] + 4))
 
 
 @pytest.fixture
@@ -125,3 +125,56 @@ def test_the_engine_says_how_long_its_sequences_are(monkeypatch):
                          host_query_lens=lens, max_query_len=max(lens))
         mixer._attention(torch.zeros(T, 64, dtype=torch.bfloat16), T, step, LayerCache(group=0), env.workspace)
         assert seen.pop() == want
+
+
+def wide_scratch(step, seqs, **more):
+    """Bytes of scratch that a step's portions ask for."""
+    asked = []
+
+    def scratch(name, shape, dtype):
+        if name == "attn.kv8_wide":
+            asked.append(shape[0] * dtype.itemsize)
+        return torch.empty(0, dtype=dtype)
+    step(seqs, scratch=scratch, **more)
+    return asked[0] if asked else 0
+
+
+TOKEN = 2 * 8 * 128 * 2            # bytes of a token's keys and values, widened
+
+
+def test_scratch_is_for_the_portions_own_keys(step):
+    """Not for the widest block table of the step."""
+    alone = wide_scratch(step, [(600, 512), (400, 400)], contexts=[600, 400])
+    assert 2 * 600 * TOKEN <= alone <= 2 * 640 * TOKEN * 1.01
+    seqs = [(131072, 1), (600, 512), (400, 400)]
+    assert wide_scratch(step, seqs, contexts=contexts(seqs)) == alone
+
+
+def test_twelve_prompts_beside_a_long_conversation_go_together(step):
+    seqs = [(131072, 1)] + [(600 - i, 600 - i) for i in range(12)]
+    assert [name for name, _ in step(seqs, contexts=contexts(seqs))] == [PORTIONS, ROWS]
+
+
+def test_scratch_of_a_window(step):
+    """512 rows behind 100000 keys see 512 + 1024 of them."""
+    seqs = [(100512, 512)]
+    assert wide_scratch(step, seqs, window=1024, contexts=contexts(seqs)) <= (512 + 1024 + 256) * TOKEN * 1.01
+    assert wide_scratch(step, seqs, window=1024) <= (512 + 1024 + 256) * TOKEN * 1.01
+    assert wide_scratch(step, seqs, contexts=contexts(seqs)) >= 100512 * TOKEN
+
+
+def test_dense_tiles_hold_what_the_rows_see():
+    for window in (1, 2, 64, 127, 128, 129, 500):
+        for rows in (1, 2, 100, 128, 129):
+            for keys in [k for k in (1, 2, 127, 128, 129, 700, 1000, 1023, 1024, 1025) if k >= rows]:
+                first = max(keys - rows - window + 1, 0)
+                assert (keys - 1) // 128 - first // 128 + 1 <= kv8.dense_tiles(rows, keys, window) <= -(-keys // 128)
+                assert kv8.dense_tiles(rows, keys, 0) == -(-keys // 128)
+
+
+def test_groups_of_portions():
+    lens, keys = [100] * 5, [128, 1280, 128, 12800, 128]
+    assert kv8.group_portions(lens, keys, 0, 10 ** 6) == [(0, 5, 100)]
+    assert kv8.group_portions(lens, keys, 0, 30) == [(0, 3, 10), (3, 4, 100), (4, 5, 1)]
+    assert kv8.group_portions(lens, keys, 0, 0) == [(i, i + 1, k // 128) for i, k in enumerate(keys)]
+    assert kv8.group_portions([0, 3], [1, 3], 0, 10) == [(0, 2, 1)]
