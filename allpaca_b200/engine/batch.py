@@ -52,10 +52,10 @@ class StepBatch:
     # (0: not known; the longest context of all stands in)
     max_decode_context_len: int = 0
     mean_context_len: int = 0
+    _contexts: Optional[List[int]] = field(default=None, repr=False)
 
     def host_contexts(self) -> List[int]:
         """Tokens that each request holds after this step."""
-        got = self.shared.get("host_contexts")
-        if got is None:
-            got = self.shared["host_contexts"] = [f + n for f, n in zip(self.host_first_position, self.host_query_lens)]
-        return got
+        if self._contexts is None:
+            self._contexts = [f + n for f, n in zip(self.host_first_position, self.host_query_lens)]
+        return self._contexts

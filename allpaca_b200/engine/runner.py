@@ -193,8 +193,12 @@ class ModelRunner:
         torch.cuda.current_stream().synchronize()
         before = library.launch_count()
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
-            gs.logits = self.model.forward(batch)
+        self.workspace.recording = True
+        try:
+            with torch.cuda.graph(graph):
+                gs.logits = self.model.forward(batch)
+        finally:
+            self.workspace.recording = False
         gs.num_kernels = library.launch_count() - before
         library.add_launches(-gs.num_kernels)            # recorded, not run
         gs.graph = graph

@@ -90,10 +90,14 @@ class Workspace:
         self.device = device
         self._buffers: Dict[str, torch.Tensor] = {}
         self._views: Dict[tuple, torch.Tensor] = {}     # (name, shape, dtype) -> the view last handed out
-        self.generation = 0          # grows whenever a buffer is replaced (its address changes)
+        self._recorded: set = set()  # buffers that were asked for while `recording`: a graph holds their addresses
+        self.recording = False       # set while a step is recorded as a graph
+        self.generation = 0          # grows whenever a buffer that a graph holds is replaced (its address changes)
 
     def get(self, name: str, shape: Sequence[int], dtype: torch.dtype) -> torch.Tensor:
         vkey = (name, tuple(shape), dtype)
+        if self.recording:
+            self._recorded.add((name, dtype))
         view = self._views.get(vkey)
         if view is not None:
             return view                  # the same shape as before: the same view of the same memory
@@ -106,7 +110,8 @@ class Workspace:
             grow = max(n, 1)
             buf = torch.empty(grow, dtype=dtype, device=self.device)
             self._buffers[key] = buf
-            self.generation += 1
+            if (name, dtype) in self._recorded:
+                self.generation += 1
             # views of the buffer this one replaces are stale
             self._views = {k: v for k, v in self._views.items() if not (k[0] == name and k[2] == dtype)}
         view = buf[:n].view(*shape)
