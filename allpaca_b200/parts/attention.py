@@ -183,7 +183,7 @@ class GroupedQueryAttention(Mixer):
             ops.attention_kv8(q, attn, cache.pages, step.block_tables[cache.group], step.token_seq, step.positions, self.nh,
                               self.nkv, self.hd, self.env.page_size, self.scale, self.window or 0, seq_start=step.seq_start,
                               query_lens=step.host_query_lens, max_context=step.max_decode_context_len or step.max_context_len,
-                              scratch=ws.get, mean_context=step.mean_context_len,
+                              scratch=ws.grow, mean_context=step.mean_context_len,
                               contexts=step.host_contexts() if step.max_query_len > 1 else None)
             return attn
         ops.attention(q, attn, cache.pages, step.block_tables[cache.group], step.token_seq,

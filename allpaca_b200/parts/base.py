@@ -22,6 +22,7 @@ names, shapes, roles) and ``load()`` receives them.  A part is registered with
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from typing import Any, Callable, Dict, List, Mapping, Optional, Sequence, Tuple
 
@@ -119,6 +120,13 @@ class Workspace:
             self._views.clear()
         self._views[vkey] = view
         return view
+
+    def grow(self, name: str, shape: Sequence[int], dtype: torch.dtype) -> torch.Tensor:
+        """:meth:`get` for a buffer that longer contexts make larger step after step: it is replaced by one at least twice as large."""
+        held = self._buffers.get(f"{name}:{dtype}")
+        if held is not None and held.numel() < math.prod(shape) < 2 * held.numel():
+            self.get(name, (2 * held.numel(),), dtype)
+        return self.get(name, shape, dtype)
 
     def bytes(self) -> int:
         return sum(b.numel() * b.element_size() for b in self._buffers.values())
