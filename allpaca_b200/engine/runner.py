@@ -86,6 +86,8 @@ class ModelRunner:
         else:
             free, _ = torch.cuda.mem_get_info(self.device)
             budget = int(free * e.gpu_memory_fraction)
+            budget -= max((g.need.scratch_bytes(e.dtype, self.max_model_len, e.max_num_batched_tokens, e.max_num_seqs)
+                           for g in self.cache_plan), default=0)
             num_pages = max(1, budget // max(1, sum(page_bytes)))
             # no more than every sequence slot at full length needs
             num_pages = min(num_pages, e.max_num_seqs * -(-self.max_model_len // e.page_size))

@@ -292,6 +292,16 @@ def group_portions(query_lens: Sequence[int], contexts: Sequence[int], window: i
     return groups + [(first, len(query_lens), widest)]
 
 
+def portions_scratch_bytes(num_kv_heads: int, head_dim: int, tokens: int, rows: int, sequences: int, window: int = 0) -> int:
+    """Bytes of scratch that portions take at most in a step of up to ``rows`` rows and ``sequences`` sequences of up to ``tokens`` tokens:
+    what one sequence needs, more only up to ``WIDE_SCRATCH``."""
+    if head_dim not in (64, 128):
+        return 0
+    tile = num_kv_heads * (4 * 128 * head_dim + 4)
+    one = dense_tiles(rows, tokens, window)
+    return -(-tile * max(one, min(sequences * one, WIDE_SCRATCH // tile)) // 16) * 16
+
+
 def _portions(q, out, cache, table, seq_start, positions, first_seq, query_lens, T, num_heads, num_kv_heads, head_dim, page_size, scale,
               window, per_tile, longest, contexts, scratch, device) -> None:
     """The sequences from ``first_seq`` on, by their ``query_lens``, of ``contexts`` keys each, or (None) some ``longest``; their rows follow

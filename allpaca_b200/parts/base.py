@@ -169,6 +169,10 @@ class CacheNeed:
             n *= int(d)
         return n * torch.empty((), dtype=self.dtype or engine_dtype).element_size()
 
+    def scratch_bytes(self, engine_dtype: torch.dtype, tokens: int, rows: int, sequences: int) -> int:
+        """Workspace that reading these pages takes beside them, where it is too much to be left to what the pages leave free."""
+        return 0
+
 
 @dataclass(frozen=True)
 class KV8Need(CacheNeed):
@@ -185,6 +189,13 @@ class KV8Need(CacheNeed):
 
     def page_bytes(self, page_size: int, engine_dtype: torch.dtype) -> int:
         return self.page_shape(page_size)[0]
+
+    def scratch_bytes(self, engine_dtype: torch.dtype, tokens: int, rows: int, sequences: int) -> int:
+        from ..ops.kv8 import portions_scratch_bytes
+        if engine_dtype != torch.bfloat16:
+            return 0
+        # (the workspace replaces the buffer by one up to twice as large as it has to be)
+        return 2 * portions_scratch_bytes(self.num_kv_heads, self.head_dim, tokens, rows, sequences, self.window or 0)
 
 
 def KVNeed(num_kv_heads: int, head_dim: int, window: Optional[int] = None) -> CacheNeed:

@@ -178,3 +178,39 @@ def test_groups_of_portions():
     assert kv8.group_portions(lens, keys, 0, 30) == [(0, 3, 10), (3, 4, 100), (4, 5, 1)]
     assert kv8.group_portions(lens, keys, 0, 0) == [(i, i + 1, k // 128) for i, k in enumerate(keys)]
     assert kv8.group_portions([0, 3], [1, 3], 0, 10) == [(0, 2, 1)]
+
+
+def test_the_most_scratch(step):
+    """No step of an engine asks for more than portions_scratch_bytes."""
+    import random
+    r = random.Random(2)
+    for i in range(60):
+        window, n, tokens = r.choice((0, 0, 700)), r.randint(1, 24), r.choice((3000, 40000, 131072))
+        seqs = []
+        for _ in range(n):
+            keys = r.randint(2, tokens)
+            seqs.append((keys, min(keys, r.randint(2, 2048 // n))))
+        most = kv8.portions_scratch_bytes(8, 128, tokens, 2048, 24, window)
+        asked = wide_scratch(step, seqs, window=window, contexts=contexts(seqs))
+        assert asked <= most <= max(131072 * TOKEN * 1.01, kv8.WIDE_SCRATCH)
+    assert kv8.portions_scratch_bytes(8, 96, 131072, 2048, 24) == 0
+
+
+def test_pages_leave_room_for_it(monkeypatch):
+    """An engine that plans its pages by the free memory keeps what portions of the longest sequence need."""
+    from allpaca_b200.config import EngineConfig
+    from allpaca_b200.engine.runner import ModelRunner
+    from allpaca_b200.models.decoder import CacheGroupPlan
+    from allpaca_b200.parts import KV8Need, KVNeed
+    free = 8 << 30
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device=None: (free, free))
+    for need, kv_dtype, room in ((KV8Need(num_kv_heads=8, head_dim=128), "fp8", 2 * 131072 * TOKEN), (KVNeed(8, 128), "auto", 0),
+                                 (KV8Need(num_kv_heads=8, head_dim=96), "fp8", 0)):
+        plan = [CacheGroupPlan(need, [0])]
+        runner = types.SimpleNamespace(
+            engine=EngineConfig(dtype=torch.bfloat16, kv_dtype=kv_dtype, page_size=16, max_num_seqs=10 ** 6), max_model_len=131072,
+            device=torch.device("meta"), model=types.SimpleNamespace(cache_plan=lambda: plan, state_bytes=lambda: [0],
+                                                                     bind_caches=lambda *a: None))
+        ModelRunner._setup_caches(runner)
+        pages = runner.num_pages * need.page_bytes(16, torch.bfloat16)
+        assert free * 0.85 - pages >= room and (room or free * 0.85 - pages < 1 << 20)
