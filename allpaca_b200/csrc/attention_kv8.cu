@@ -132,7 +132,8 @@ AP_EXPORT int ap_attention_kv8_rows(const void* q, void* out, int dtype, const v
     AP_REQUIRE(num_pages >= 0 && num_pages < (1LL << 31) && page_bytes == kv8_page_bytes(nkv, P, HD),
                "attention_kv8: the pages do not match the heads");
     AP_REQUIRE(((uintptr_t)cache & 15) == 0, "attention_kv8: the cache must be 16-byte aligned");
-    AP_REQUIRE((long long)max_blocks * P < (1LL << 31), "attention_kv8: the block table names more than 2^31 keys");
+    // (a chunk's last key may lie K8_CHUNK past a row's)
+    AP_REQUIRE((long long)max_blocks * P < (1LL << 31) - 2 * K8_CHUNK, "attention_kv8: the block table names some 2^31 keys or more");
     if (T == 0) return AP_OK;
     const dim3 grid(T, nh);
 #define K8_ROWS(TT)                                                                                                          \

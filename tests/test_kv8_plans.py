@@ -214,3 +214,15 @@ def test_pages_leave_room_for_it(monkeypatch):
         ModelRunner._setup_caches(runner)
         pages = runner.num_pages * need.page_bytes(16, torch.bfloat16)
         assert free * 0.85 - pages >= room and (room or free * 0.85 - pages < 1 << 20)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 80])
+def test_block_tables_whose_keys_an_index_cannot_hold(hd):
+    """The entry points refuse tables that name nearly 2^31 keys or more (checked before anything is launched: no rows here)."""
+    from allpaca_b200.ops import library
+    lib, nkv = library.attention(hd), 1
+    entry = lib.ap_attention_kv8_rows
+    for P, blocks, fine in ((16, 1 << 20, True), (1, 2 ** 31 - 1, False), (16, (1 << 27) - 1, False), (1, 2 ** 31 - 1 - 512, True),
+                            (2 ** 30, 1, True), (2 ** 30, 2, False)):
+        rc = entry(0, 0, 1, 0, 1, kv8.kv8_page_bytes(nkv, P, hd), 0, blocks, 1, 0, 0, 0, 2, nkv, hd, P, 0.1, 0, 0)
+        assert (rc == 0) is fine, (P, blocks)
