@@ -20,12 +20,16 @@
 // the 16 rows, and it is the queries and the weights that are split into two e4m3 numbers, x = hi + lo / 16, side by side in the
 // eight columns: four query rows to a product.  That keeps the eight significant bits of bfloat16 (hi is off by half of the last of
 // four bits, and so much needs four bits again).  Queries are scaled by a power of two to a row (numbers down to 2^-15 of the largest keep all
-// eight bits), weights lie between 0 and 256.
+// eight bits).  Weights, with their values' scales, lie between 0 and 256, off by 2^-8 of themselves or by 2^-14: so they are taken relative to
+// a reference that follows the largest of each 32 keys, up at once, down when those lie 2^4 below it (rescaling the sums then, 1 to 1.5 % of
+// the time).  Against one maximum for all keys, weights of less than 2^-22 of it were lost, and of 70000 keys behind one that took nearly
+// all of the softmax a tenth of their sum.
 //
 //   t_j = log2(e) scale 2^a_j (q . c_j),   m >= t_j + b_j,   l = sum_j 2^(t_j - m),   out = sum_j 2^(t_j + b_j - m) d_j / l
 //
 // with scales 2^a_j of keys and 2^b_j of values: a maximum over what meets the 8-bit numbers keeps the largest products exact
-// however values differ in size, and with b_j between -60 and 40 neither sum leaves the range of 32-bit numbers.
+// however values differ in size, and with b_j between -60 and 40, and the reference no more than 2^30 below the maximum, neither sum leaves the
+// range of 32-bit numbers.
 //
 // The key is the summed index of the second product, so four keys' numbers of a column have to lie side by side in a register: a
 // transposing ldmatrix brings two columns of two keys, two byte permutes sort two such registers.  Which key is which row of a tile
@@ -55,6 +59,8 @@
 #define K8D_PAIR_COST 4                        // tiles
 #define K8D_FEW_PARTS 4                        // of a pair, up to which one warp adds them up
 #define K8D_MAX_ROWS 512                       // of a launch
+#define K8D_NEAR 4.f                           // powers of two that a tile's largest weight may lie below what its weights are relative to,
+#define K8D_FALL 30.f                          // and that this may lie below the largest of all
 // Rows lie in shared memory as TMA leaves them: `BOX` bytes to a row, the 16-byte chunks of 8 (4, 2) rows swizzled where a box is 128 (64,
 // 32) bytes wide, so that eight rows of one ldmatrix lie in different banks; other head sizes take what conflicts they have.
 #define BOX (HD % 128 == 0 ? 128 : HD)
@@ -652,10 +658,10 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
         }
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&q_empty[k & 1]);
-        float o[NT][CHUNKS][4], m[NT], l[NT];
+        float o[NT][CHUNKS][4], m[NT], l[NT], top[NT];         // m: what the sums are relative to; top: the largest so far
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            m[n] = -INFINITY;
+            m[n] = top[n] = -INFINITY;
             l[n] = 0.f;
 #pragma unroll
             for (int i = 0; i < CHUNKS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
@@ -732,11 +738,18 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
                     t[i] = kb[i] ? t[i] : -INFINITY;
                     mx = fmaxf(mx, t[i] + ((float)vb[i] - 127.f));
                 }
-                if (__any_sync(0xffffffffu, mx > m[n])) {
+                // (heads, four of them, with a key that is near the reference from below)
+                uint32_t near = __ballot_sync(0xffffffffu, mx >= m[n] - K8D_NEAR);
+                near |= near >> 16;
+                near |= near >> 8;
+                near |= near >> 4;
+                if (__any_sync(0xffffffffu, mx > m[n]) || (near & 0xfu) != 0xfu) {
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float m_new = fmaxf(m[n], mx);
+                    top[n] = fmaxf(top[n], mx);
+                    float m_new = fmaxf(m[n], mx);
+                    if (mx < m[n] - K8D_NEAR && mx > -INFINITY) m_new = fmaxf(mx, top[n] - K8D_FALL);
                     const float alpha = m_new == -INFINITY ? 0.f : k8_exp2(m[n] - m_new);
                     m[n] = m_new;
                     l[n] *= alpha;
