@@ -330,13 +330,18 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
                   query_lens: Optional[Sequence[int]] = None, max_context: int = 0, scratch=None,
                   mean_context: int = 0, contexts: Optional[Sequence[int]] = None) -> None:
     """Causal attention of every row of ``q [T, nh*hd]`` over its sequence's keys in the 8-bit cache; arguments as for
-    :func:`attention`, with ``page_size`` beside the flat pages (``max_context`` and ``mean_context`` only say how to cut the work).
+    :func:`attention`, with ``page_size`` beside the flat pages.  ``max_context`` and ``mean_context`` only say how to cut the work.
     ``contexts`` (host, one to a sequence of ``query_lens``): the sequences' keys, the newest row's among them (none may have
-    more); without it portions are planned by ``max_context`` where no sequence brings one row, else by the width of the block table, and their
-    scratch is as wide as the table.  Scores, softmax and sums are 32-bit.  A row sees the keys at and before its position (the last ``window`` of them, 0: all) whose
-    page is there; one that sees none gets zeros.  A key that is not finite makes the rows that see it NaN, a value their columns of it, no
-    other row.  The rows of a sequence follow one another and so do their positions; ``out`` is
-    another tensor than ``q``.  Calls that may run at the same time need scratch of their own (None: each allocates it)."""
+    more).  Without it portions are planned by ``max_context`` where no sequence brings one row, else by the width of the block
+    table, and their scratch is as wide as the table.
+
+    Scores, softmax and sums are 32-bit; in bfloat16 a weight is rounded to eight bits before it meets its value (single rows: together
+    with the value's scale, and to 2^-18 of the largest such weight among 32 neighbours).  A row sees the keys at and before its
+    position (the last ``window`` of them, 0: all) whose page is there; one that sees none gets zeros.  A key that is not finite makes
+    the rows that see it NaN, a value their columns of it, no other row.
+
+    The rows of a sequence follow one another and so do their positions; ``out`` is another tensor than ``q``.  Calls that may run
+    at the same time need scratch of their own (None: each allocates it)."""
     what = "attention_kv8"
     device, T, cache, table = _take_cache(what, cache_layer, num_kv_heads, head_dim, page_size, positions, token_seq, block_table)
     code = _CODES.get(q.dtype)
