@@ -10,7 +10,7 @@ from __future__ import annotations
 import functools
 import itertools
 import random
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -248,7 +248,8 @@ def rows_are_faster(rows_us: float, sequences: int, longest: int, numbers: int, 
 WIDE_SCRATCH = 1 << 30
 
 
-def step_lengths(query_lens: Sequence[int], ones: int, contexts: Optional[Sequence[int]], max_context: int, mean_context: int,
+@functools.lru_cache(maxsize=256)
+def step_lengths(query_lens: Tuple[int, ...], ones: int, contexts: Optional[Tuple[int, ...]], max_context: int, mean_context: int,
                  widest: int):
     """What a step with portions from sequence ``ones`` on is planned by: (longest context from there on, longest and average context of all
     rows).  Where ``contexts`` does not say, ``max_context`` counts only if there are no one-row sequences that it may stand for,
@@ -261,16 +262,17 @@ def step_lengths(query_lens: Sequence[int], ones: int, contexts: Optional[Sequen
     return max(1, min(max(contexts[ones:]), widest)), max(1, longest), max(1, min(mean, longest))
 
 
-def _row_by_row(query_lens, per_tile, num_heads, num_kv_heads, head_dim, window, longest, device) -> bool:
+@functools.lru_cache(maxsize=256)
+def _row_by_row(plan, faster, query_lens, per_tile, num_heads, num_kv_heads, head_dim, window, longest, device) -> bool:
     """Whether the portions of ``query_lens`` go to the kernel for single rows."""
     if window:
         longest = min(longest, window + max(query_lens))
     _, sms, clusters, sets = _machine(device, num_heads, num_kv_heads, head_dim)
     rows_us = _rows_cost(sum(query_lens) * sets, -(-longest // 64), -(-longest // 64), sms, clusters)[0]
-    query_tiles, ctas, slices = plan_portions(query_lens, per_tile, num_kv_heads, longest - max(query_lens) // 2, sms)
+    query_tiles, ctas, slices = plan(query_lens, per_tile, num_kv_heads, longest - max(query_lens) // 2, sms)
     at_once = slices * (2 if slices > 1 and max(query_lens) <= per_tile else 1)
-    return rows_are_faster(rows_us, len(query_lens), longest, num_kv_heads * head_dim, query_tiles, at_once,
-                           -(-ctas * num_kv_heads * slices // (sms * (3 - query_tiles))))
+    return faster(rows_us, len(query_lens), longest, num_kv_heads * head_dim, query_tiles, at_once,
+                  -(-ctas * num_kv_heads * slices // (sms * (3 - query_tiles))))
 
 
 def dense_tiles(rows: int, keys: int, window: int) -> int:
@@ -302,25 +304,34 @@ def portions_scratch_bytes(num_kv_heads: int, head_dim: int, tokens: int, rows: 
     return -(-tile * max(one, min(sequences * one, WIDE_SCRATCH // tile)) // 16) * 16
 
 
+@functools.lru_cache(maxsize=256)
+def _portions_plan(lib, plan, most, sms, query_lens, contexts, longest, widest, window, per_tile, num_kv_heads):
+    """(bytes of scratch, [(first sequence, sequences, dense tiles of each, query tiles to a CTA, CTAs to a KV head, key slices), ...]), the same
+    for every layer of a step."""
+    keys = [widest] * len(query_lens) if contexts is None else [max(1, min(c, widest)) for c in contexts]
+    groups, need = [], 0
+    for at, end, tiles in group_portions(query_lens, keys, window, most // lib.ap_attention_kv8_tcgen05_scratch(1, num_kv_heads)):
+        lens, seen = query_lens[at:end], longest if contexts is None else max(keys[at:end])
+        if window:
+            seen = min(seen, window + max(lens))
+        groups.append((at, end - at, tiles, *plan(lens, per_tile, num_kv_heads, seen - max(lens) // 2, sms)))
+        need = max(need, lib.ap_attention_kv8_tcgen05_scratch((end - at) * tiles, num_kv_heads))
+    return need, groups
+
+
 def _portions(q, out, cache, table, seq_start, positions, first_seq, query_lens, T, num_heads, num_kv_heads, head_dim, page_size, scale,
               window, per_tile, longest, contexts, scratch, device) -> None:
     """The sequences from ``first_seq`` on, by their ``query_lens``, of ``contexts`` keys each, or (None) some ``longest``; their rows follow
     those of the sequences before."""
     (blocks, width, _), lib = table, library.attention(head_dim)
-    widest = width * page_size
-    keys = [widest] * len(query_lens) if contexts is None else [max(1, min(c, widest)) for c in contexts]
-    groups = group_portions(query_lens, keys, window, WIDE_SCRATCH // lib.ap_attention_kv8_tcgen05_scratch(1, num_kv_heads))
-    need = lib.ap_attention_kv8_tcgen05_scratch(max((end - at) * tiles for at, end, tiles in groups), num_kv_heads)
+    need, groups = _portions_plan(lib, plan_portions, WIDE_SCRATCH, _sms(device), query_lens, contexts, longest, width * page_size, window,
+                                  per_tile, num_kv_heads)
     buf = scratch("attn.kv8_wide", (need // 2,), torch.bfloat16) if scratch is not None else \
         torch.empty(need // 2, dtype=torch.bfloat16, device=q.device)
-    for at, end, tiles in groups:
-        lens, most = query_lens[at:end], longest if contexts is None else max(keys[at:end])
-        if window:
-            most = min(most, window + max(lens))
-        query_tiles, ctas, slices = plan_portions(lens, per_tile, num_kv_heads, most - max(lens) // 2, _sms(device))
+    for at, sequences, tiles, query_tiles, ctas, slices in groups:
         if ctas:
             call(lib, "ap_attention_kv8_tcgen05", q.data_ptr(), out.data_ptr(), *cache, blocks + 4 * (first_seq + at) * width, width,
-                 seq_start.data_ptr() + 4 * (first_seq + at), positions.data_ptr(), len(lens), T, num_heads, num_kv_heads, head_dim,
+                 seq_start.data_ptr() + 4 * (first_seq + at), positions.data_ptr(), sequences, T, num_heads, num_kv_heads, head_dim,
                  page_size, float(scale), int(window), query_tiles, ctas, slices, tiles, buf.data_ptr(), need, stream_handle())
 
 
@@ -371,10 +382,11 @@ def attention_kv8(q: torch.Tensor, out: torch.Tensor, cache_layer: torch.Tensor,
             # (as many sequences as rows: one each, or none and several here and there, which the rows' own metadata says as well)
             ones = next((i for i, n in enumerate(query_lens) if n != 1), len(query_lens)) if len(query_lens) != T else T
             if ones < len(query_lens):
+                query_lens, contexts = tuple(query_lens), tuple(contexts) if contexts is not None else None
                 behind, all_longest, all_mean = step_lengths(query_lens, ones, contexts, max_context, mean_context, widest)
                 per_tile = _portions_taken(num_heads, num_kv_heads, head_dim, page_size) if scale > 0 else 0
-                if per_tile and not (T <= 512 and _row_by_row(query_lens[ones:], per_tile, num_heads, num_kv_heads, head_dim, window,
-                                                              behind, device)):
+                if per_tile and not (T <= 512 and _row_by_row(plan_portions, rows_are_faster, query_lens[ones:], per_tile, num_heads,
+                                                              num_kv_heads, head_dim, window, behind, device)):
                     _portions(q, out, cache, table, seq_start, positions, ones, query_lens[ones:], T, num_heads, num_kv_heads, head_dim,
                               page_size, scale, window, per_tile, behind, None if contexts is None else contexts[ones:], scratch, device)
                     rows = ones

@@ -22,7 +22,7 @@ class Library:
 @pytest.fixture
 def step(monkeypatch):
     """step(seqs of (keys, rows), ...) -> [(entry point, how it is planned)]."""
-    caches = [kv8._machine, kv8._single_rows_taken, kv8._portions_taken, kv8._scratch_bytes]
+    caches = [kv8._machine, kv8._single_rows_taken, kv8._portions_taken, kv8._scratch_bytes, kv8._row_by_row, kv8._portions_plan]
     for f in caches:
         f.cache_clear()
     calls, planned = [], []
@@ -47,6 +47,8 @@ def step(monkeypatch):
     def run(seqs, **more):
         nh, nkv, hd, P = HEADS
         del calls[:], planned[:]
+        for f in caches:                                   # (a plan that was made before is not made again)
+            f.cache_clear()
         T, lens = sum(n for _, n in seqs), [n for _, n in seqs]
         ints = lambda n: torch.zeros(n, dtype=torch.int32)   # noqa: E731
         q = torch.zeros((T, nh * hd), dtype=torch.bfloat16)
