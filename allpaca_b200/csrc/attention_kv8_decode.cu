@@ -11,10 +11,10 @@
 // their own.  Few pairs get a cluster of CTAs each instead, whose parts meet in distributed shared memory.
 //
 // Bound by memory while it streams, at 5.8 to 6.4 TB/s with pages scattered: 64 rows of 2048 keys (8 KV heads of 128: 270 MB, floor 41.9 us at
-// the copy rate) take 54.6 us, of which 5.5 pass before the first tile is there (positions, block table and tile are read one after
-// the other) and 3 after the last.  One row of 32768 keys (floor 10.5) takes 25.7: 5.5, 10.5 of streaming, 9 until parts are written, seen
-// and added up.  Ragged rows (64 of 150 to 4096 keys, floor 24.7) take 47.8: each pair costs four tiles' time beside its own.  Heads of
-// 64 (64 rows of 4096 keys: 71, floor 42.2) are bound by what the working warps do per tile, which does not shrink with the head.
+// the copy rate) take 57.5 us, of which 5.5 pass before the first tile is there (positions, block table and tile are read one after
+// the other) and 3 after the last.  One row of 32768 keys (floor 10.5) takes 24.3: 5.5, 10.5 of streaming, the rest until parts are written,
+// seen and added up.  Ragged rows (64 of 150 to 4096 keys, floor 24.7) take 47.4: each pair costs four tiles' time beside its own.  Heads of
+// 64 (64 rows of 4096 keys: 75.5, floor 42.2) are bound by what the working warps do per tile, which does not shrink with the head.
 //
 // The numbers are never widened: the products are e4m3 x e4m3 (mma.sync m16n8k32) with the keys, and the columns of the values, as
 // the 16 rows, and it is the queries and the weights that are split into two e4m3 numbers, x = hi + lo / 16, side by side in the
@@ -412,7 +412,7 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
             }
 #pragma unroll 1
             for (int i = warp; i < nparts; i += CWARPS) {
-                    float2 ml[4 * NT];
+                float2 ml[4 * NT];
                 float4 po[4 * NT];
 #pragma unroll
                 for (int h = 0; h < 4 * NT; ++h) fetch(i, min(h, p.heads - 1), d, ml[h], po[h]);      // (heads past the last one: the last one again)
@@ -490,64 +490,63 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == QUERY_WARP) {
-
         // ---- queries: of every pair ahead of its turn, split and in the order of the products' operands ----
         int k = 0;
         for (int seg = 0; seg < 3; ++seg) {
-        K8dAt at = work.at(min(run_from(seg), W - 1));
-        for (int w = run_from(seg); w < run_to(seg); ++k) {
-            const int kvh = (j0 + at.j) / p.n_chunks, chunk = j0 + at.j - kvh * p.n_chunks;
-            const int head0 = kvh * group + chunk * p.heads, nheads = min(p.heads, group - chunk * p.heads);
-            // column g of product n is query head 4 n + g / 2, its high half where g is even
-            uint32_t words[NT][CHUNKS];
-            float factor[NT];
+            K8dAt at = work.at(min(run_from(seg), W - 1));
+            for (int w = run_from(seg); w < run_to(seg); ++k) {
+                const int kvh = (j0 + at.j) / p.n_chunks, chunk = j0 + at.j - kvh * p.n_chunks;
+                const int head0 = kvh * group + chunk * p.heads, nheads = min(p.heads, group - chunk * p.heads);
+                // column g of product n is query head 4 n + g / 2, its high half where g is even
+                uint32_t words[NT][CHUNKS];
+                float factor[NT];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int hq = 4 * n + (g >> 1);
-                const bf16* qr = p.q + ((size_t)(row0 + at.row) * p.nh + head0 + (hq < nheads ? hq : 0)) * HD + c * 4;
-                uint2 raw[CHUNKS];
-                uint32_t amax = 0;
+                for (int n = 0; n < NT; ++n) {
+                    const int hq = 4 * n + (g >> 1);
+                    const bf16* qr = p.q + ((size_t)(row0 + at.row) * p.nh + head0 + (hq < nheads ? hq : 0)) * HD + c * 4;
+                    uint2 raw[CHUNKS];
+                    uint32_t amax = 0;
 #pragma unroll
-                for (int i = 0; i < CHUNKS; ++i) raw[i] = hq < nheads ? *reinterpret_cast<const uint2*>(qr + i * 16) : make_uint2(0u, 0u);
+                    for (int i = 0; i < CHUNKS; ++i) raw[i] = hq < nheads ? *reinterpret_cast<const uint2*>(qr + i * 16) : make_uint2(0u, 0u);
 #pragma unroll
-                for (int i = 0; i < CHUNKS; ++i) {
-                    const uint32_t x[4] = {raw[i].x << 16, raw[i].x & 0xffff0000u, raw[i].y << 16, raw[i].y & 0xffff0000u};
+                    for (int i = 0; i < CHUNKS; ++i) {
+                        const uint32_t x[4] = {raw[i].x << 16, raw[i].x & 0xffff0000u, raw[i].y << 16, raw[i].y & 0xffff0000u};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t m = x[e] & 0x7fffffffu;
-                        amax = max(amax, m < 0x7f800000u ? m : 0u);
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t m = x[e] & 0x7fffffffu;
+                            amax = max(amax, m < 0x7f800000u ? m : 0u);
+                        }
+                    }
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    // 2^e with e the smallest exponent under which no number exceeds 448 (kept where 2^e and 2^-e are normal numbers)
+                    const int e = min(max((int)(amax >> 23) - 135 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0), -120), 120);
+                    const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+                    factor[n] = __shfl_sync(0xffffffffu, p.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23), 8 * c);   // of head 4 n + c
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; ++i) {
+                        float x[4] = {__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xffff0000u),
+                                      __uint_as_float(raw[i].y << 16), __uint_as_float(raw[i].y & 0xffff0000u)};
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) x[y] = fmaf(x[y], inv, x[y] - x[y]);       // NaN where not finite
+                        uint32_t h, l;
+                        k8_split(x[0], x[1], x[2], x[3], h, l);
+                        words[n][i] = g & 1 ? l : h;
                     }
                 }
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                // 2^e with e the smallest exponent under which no number exceeds 448 (kept where 2^e and 2^-e are normal numbers)
-                const int e = min(max((int)(amax >> 23) - 135 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0), -120), 120);
-                const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-                factor[n] = __shfl_sync(0xffffffffu, p.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23), 8 * c);   // of head 4 n + c
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&q_empty[k & 1], (uint32_t)((k >> 1) & 1) ^ 1))) give_up();
 #pragma unroll
-                for (int i = 0; i < CHUNKS; ++i) {
-                    float x[4] = {__uint_as_float(raw[i].x << 16), __uint_as_float(raw[i].x & 0xffff0000u),
-                                  __uint_as_float(raw[i].y << 16), __uint_as_float(raw[i].y & 0xffff0000u)};
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) x[y] = fmaf(x[y], inv, x[y] - x[y]);       // NaN where not finite
-                    uint32_t h, l;
-                    k8_split(x[0], x[1], x[2], x[3], h, l);
-                    words[n][i] = g & 1 ? l : h;
+                    for (int i = 0; i < CHUNKS; ++i) s_query[k & 1][n][i][lane] = words[n][i];
+                    s_query[k & 1][n][CHUNKS][lane] = __float_as_uint(factor[n]);
                 }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&q_full[k & 1]);
+                w += at.end - at.tile;
+                at.tile = at.end - 1;
+                work.next(at, 1);
             }
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(&q_empty[k & 1], (uint32_t)((k >> 1) & 1) ^ 1))) give_up();
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int i = 0; i < CHUNKS; ++i) s_query[k & 1][n][i][lane] = words[n][i];
-                s_query[k & 1][n][CHUNKS][lane] = __float_as_uint(factor[n]);
-            }
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&q_full[k & 1]);
-            w += at.end - at.tile;
-            at.tile = at.end - 1;
-            work.next(at, 1);
-        }
         }
     } else if (warp == MERGE_WARP) {
         // ---- results: the working warps' sums of a pair are added up while they are at the next one ----
@@ -580,31 +579,31 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
         // (once on nothing, while the first tiles are on their way: a function's first call waits for its instructions)
         k8d_combine<NT>(merge, 0, nullptr, nullptr);
         for (int seg = 0; seg < 3; ++seg) {
-        K8dAt at = work.at(min(run_from(seg), W - 1));
-        for (int w = run_from(seg); w < run_to(seg); ph ^= 1) {
-            const int kvh = (j0 + at.j) / p.n_chunks, chunk = j0 + at.j - kvh * p.n_chunks;
-            const int head0 = kvh * group + chunk * p.heads, nheads = min(p.heads, group - chunk * p.heads);
-            const int item0 = w - at.tile, item1 = item0 + at.end;
-            const bool whole = item0 >= lo && item1 <= hi;
-            bf16* out = p.out + ((size_t)(row0 + at.row) * p.nh + head0) * HD;
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(&dumped, ph))) give_up();
-            float* part = CL ? own_part : p.parts + ((size_t)blockIdx.x * 2 + (item0 >= lo ? 1 : 0)) * p.heads * XROW;
-            k8d_combine<NT>(merge, nheads, out, whole ? nullptr : part);
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&taken);
-            if (!CL && !whole) {
-                const int nparts = work.cta_of(item1 - 1) - work.cta_of(item0) + 1;
-                say(item0);
-                if (nparts > K8D_FEW_PARTS) {
-                    late[n_late++] = {item0, nparts, nheads, out};
-                } else if (all_there(item0, nparts)) {
-                    k8d_add_few<NT>(p.parts, work.cta_of(item0), nparts, p.heads, nheads, out);
+            K8dAt at = work.at(min(run_from(seg), W - 1));
+            for (int w = run_from(seg); w < run_to(seg); ph ^= 1) {
+                const int kvh = (j0 + at.j) / p.n_chunks, chunk = j0 + at.j - kvh * p.n_chunks;
+                const int head0 = kvh * group + chunk * p.heads, nheads = min(p.heads, group - chunk * p.heads);
+                const int item0 = w - at.tile, item1 = item0 + at.end;
+                const bool whole = item0 >= lo && item1 <= hi;
+                bf16* out = p.out + ((size_t)(row0 + at.row) * p.nh + head0) * HD;
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&dumped, ph))) give_up();
+                float* part = CL ? own_part : p.parts + ((size_t)blockIdx.x * 2 + (item0 >= lo ? 1 : 0)) * p.heads * XROW;
+                k8d_combine<NT>(merge, nheads, out, whole ? nullptr : part);
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&taken);
+                if (!CL && !whole) {
+                    const int nparts = work.cta_of(item1 - 1) - work.cta_of(item0) + 1;
+                    say(item0);
+                    if (nparts > K8D_FEW_PARTS) {
+                        late[n_late++] = {item0, nparts, nheads, out};
+                    } else if (all_there(item0, nparts)) {
+                        k8d_add_few<NT>(p.parts, work.cta_of(item0), nparts, p.heads, nheads, out);
+                    }
                 }
+                w = item1;
+                at.tile = at.end - 1;
+                work.next(at, 1);
             }
-            w = item1;
-            at.tile = at.end - 1;
-            work.next(at, 1);
-        }
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -624,229 +623,230 @@ attention_kv8_decode_kernel(const __grid_constant__ CUtensorMap tmap, const __gr
             if (lane == 0) tc::mbar_arrive(&taken);
         }
     } else {
-    // ---- working: warps 2 i and 2 i + 1 take the two halves of every fourth tile (LANES) ----
-    const int half = warp & 1, turn = warp >> 1;
-    const int rows_shift = p.P < TILE ? p.P_shift : 6;     // rows of a page in a tile
-    // rows of the tile that this lane's addresses of ldmatrix name (see above: row r of a product is key 2 r and 2 r + 1)
-    const int r8 = lane & 7, mat = lane >> 3;
-    const int key_a = 2 * r8 + (r8 >= 4 ? 1 : 0), key_b = 2 * r8 + (r8 >= 4 ? 0 : 1);
-    const int k_key = half * 32 + (mat & 1 ? key_b : key_a);
-    const int v_key = half * 32 + (mat & 1) * 16 + (mat & 2 ? 8 + (r8 ^ 1) : r8);
-    const int my_a = half * 32 + 2 * g + (g >= 4 ? 1 : 0), my_b = half * 32 + 2 * g + (g >= 4 ? 0 : 1);   // and + 16
-    bool ok = true;
-    int s = 0;                                             // stage and phase of tile `w`
-    uint32_t ph = 0;
-    int k = 0, v = 0, n_late = 0, late0 = 0, late1 = 0, parts0 = 0, parts1 = 0;
-    for (int seg = 0; seg < 3; ++seg) {
-    K8dAt at = work.at(min(run_from(seg), W - 1));
-    for (int w = run_from(seg); w < run_to(seg); ++k) {
-        // one pair, or the part of it that is this CTA's
-        const int item0 = w - at.tile, item1 = item0 + at.end, stop = item1 < hi ? item1 : hi;
-        const int last = s_last[at.row], first = k8d_first(p, last);
-        if (ok && !__all_sync(0xffffffffu, tc::mbar_wait(&q_full[k & 1], (uint32_t)((k >> 1) & 1)))) {
-            give_up();
-            ok = false;
-        }
-        uint32_t qf[NT][CHUNKS + 1];
-        float rowfac[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int i = 0; i < CHUNKS; ++i) qf[n][i] = s_query[k & 1][n][i][lane];
-            qf[n][CHUNKS] = 0u;
-            rowfac[n] = __uint_as_float(s_query[k & 1][n][CHUNKS][lane]);
-        }
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&q_empty[k & 1]);
-        float o[NT][CHUNKS][4], m[NT], l[NT], top[NT];         // m: what the sums are relative to; top: the largest so far
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            m[n] = top[n] = -INFINITY;
-            l[n] = 0.f;
-#pragma unroll
-            for (int i = 0; i < CHUNKS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-        }
-        for (; w < stop; ++w, ++v) {
-            const int st = s;
-            const uint32_t sp = ph;
-            if (++s == p.stages) { s = 0; ph ^= 1; }
-            const int tile = w - item0;
-            if ((v & (LANES - 1)) != turn) continue;
-            if (ok && !__all_sync(0xffffffffu, tc::mbar_wait(&full[st], sp))) {
-                give_up();
-                ok = false;
-            }
-            if (!ok) continue;
-            uint8_t* stage = smem + (size_t)st * STAGE_BYTES;
-            const uint32_t base = tc::smem_addr(stage);
-            float sc[NT][2][4];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) sc[n][t][0] = sc[n][t][1] = sc[n][t][2] = sc[n][t][3] = 0.f;
-#pragma unroll
-                for (int i = 0; i < CHUNKS; i += 2) {
-                    uint32_t a[4];
-                    if (i + 1 < CHUNKS) k8_ldmatrix(a, base + k8_at(k_key + t * 16, i + (mat >> 1), rows_shift, false));
-                    else k8_ldmatrix_x2(a, base + k8_at(k_key + t * 16, i, rows_shift, false));
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) k8_mma(sc[n][t], a, qf[n][i], qf[n][i + 1]);
+        // ---- working: warps 2 i and 2 i + 1 take the two halves of every fourth tile (LANES) ----
+        const int half = warp & 1, turn = warp >> 1;
+        const int rows_shift = p.P < TILE ? p.P_shift : 6;     // rows of a page in a tile
+        // rows of the tile that this lane's addresses of ldmatrix name (see above: row r of a product is key 2 r and 2 r + 1)
+        const int r8 = lane & 7, mat = lane >> 3;
+        const int key_a = 2 * r8 + (r8 >= 4 ? 1 : 0), key_b = 2 * r8 + (r8 >= 4 ? 0 : 1);
+        const int k_key = half * 32 + (mat & 1 ? key_b : key_a);
+        const int v_key = half * 32 + (mat & 1) * 16 + (mat & 2 ? 8 + (r8 ^ 1) : r8);
+        const int my_a = half * 32 + 2 * g + (g >= 4 ? 1 : 0), my_b = half * 32 + 2 * g + (g >= 4 ? 0 : 1);   // and + 16
+        bool ok = true;
+        int s = 0;                                             // stage and phase of tile `w`
+        uint32_t ph = 0;
+        int k = 0, v = 0, n_late = 0, late0 = 0, late1 = 0, parts0 = 0, parts1 = 0;
+        for (int seg = 0; seg < 3; ++seg) {
+            K8dAt at = work.at(min(run_from(seg), W - 1));
+            for (int w = run_from(seg); w < run_to(seg); ++k) {
+                // one pair, or the part of it that is this CTA's
+                const int item0 = w - at.tile, item1 = item0 + at.end, stop = item1 < hi ? item1 : hi;
+                const int last = s_last[at.row], first = k8d_first(p, last);
+                if (ok && !__all_sync(0xffffffffu, tc::mbar_wait(&q_full[k & 1], (uint32_t)((k >> 1) & 1)))) {
+                    give_up();
+                    ok = false;
                 }
-            }
-            // scale bytes of this lane's keys: 2 g and 2 g + 1 (the other way round from g = 4 on), 16 further on the same; 0 where there
-            // is no page
-            uint32_t kb[4], vb[4];
-            {
-                const uint8_t* bytes = scales + st * SCALE_BYTES;
+                uint32_t qf[NT][CHUNKS + 1];
+                float rowfac[NT];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const uint32_t k2 = *reinterpret_cast<const uint16_t*>(bytes + half * 32 + t * 16 + 2 * g);
-                    const uint32_t v2 = *reinterpret_cast<const uint16_t*>(bytes + TILE + half * 32 + t * 16 + 2 * g);
-                    const uint32_t k0 = k2 & 0xffu, k1 = k2 >> 8, v0 = v2 & 0xffu, v1 = v2 >> 8;
-                    kb[2 * t] = g >= 4 ? k1 : k0;
-                    kb[2 * t + 1] = g >= 4 ? k0 : k1;
-                    vb[2 * t] = g >= 4 ? v1 : v0;
-                    vb[2 * t + 1] = g >= 4 ? v0 : v1;
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; ++i) qf[n][i] = s_query[k & 1][n][i][lane];
+                    qf[n][CHUNKS] = 0u;
+                    rowfac[n] = __uint_as_float(s_query[k & 1][n][CHUNKS][lane]);
                 }
-            }
-            const int key0 = (first / TILE + tile) * TILE + half * 32;
-            const bool inside = key0 >= first && key0 + 31 <= last;
-            const bool every = __all_sync(0xffffffffu, inside && kb[0] && kb[1] && kb[2] && kb[3]);
-            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-            if (!every) {
-                // keys before the first, behind the last, or without a page do not count, and what lies in the place of their values must not meet
-                // a weight of zero: it may be NaN.  (keep0, keep1: a byte to a key of the second product's operand in this lane)
-                uint32_t keep = 0u;
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&q_empty[k & 1]);
+                float o[NT][CHUNKS][4], m[NT], l[NT], top[NT];         // m: what the sums are relative to; top: the largest so far
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int kpos = key0 - half * 32 + (i & 1 ? my_b : my_a) + (i >> 1) * 16;
-                    if (kpos < first || kpos > last) kb[i] = 0u;
-                    if (!kb[i]) vb[i] = 0u;
-                    keep |= kb[i] ? 0xffu << (8 * i) : 0u;
+                for (int n = 0; n < NT; ++n) {
+                    m[n] = top[n] = -INFINITY;
+                    l[n] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
                 }
-                keep0 = __shfl_sync(0xffffffffu, keep, 4 * c);
-                keep1 = __shfl_sync(0xffffffffu, keep, 4 * c + 16);
-            }
-            uint32_t b0[NT], b1[NT];
+                for (; w < stop; ++w, ++v) {
+                    const int st = s;
+                    const uint32_t sp = ph;
+                    if (++s == p.stages) { s = 0; ph ^= 1; }
+                    const int tile = w - item0;
+                    if ((v & (LANES - 1)) != turn) continue;
+                    if (ok && !__all_sync(0xffffffffu, tc::mbar_wait(&full[st], sp))) {
+                        give_up();
+                        ok = false;
+                    }
+                    if (!ok) continue;
+                    uint8_t* stage = smem + (size_t)st * STAGE_BYTES;
+                    const uint32_t base = tc::smem_addr(stage);
+                    float sc[NT][2][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float t[4], mx = -INFINITY;
+                    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float* q2 = sc[n][i >> 1] + 2 * (i & 1);
-                    t[i] = fmaf(q2[1], 0.0625f, q2[0]) * (rowfac[n] * kv8_scale(kb[i]));
-                    t[i] = kb[i] ? t[i] : -INFINITY;
-                    mx = fmaxf(mx, t[i] + ((float)vb[i] - 127.f));
-                }
-                // (heads, four of them, with a key that is near the reference from below)
-                uint32_t near = __ballot_sync(0xffffffffu, mx >= m[n] - K8D_NEAR);
-                near |= near >> 16;
-                near |= near >> 8;
-                near |= near >> 4;
-                if (__any_sync(0xffffffffu, mx > m[n]) || (near & 0xfu) != 0xfu) {
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    top[n] = fmaxf(top[n], mx);
-                    float m_new = fmaxf(m[n], mx);
-                    if (mx < m[n] - K8D_NEAR && mx > -INFINITY) m_new = fmaxf(mx, top[n] - K8D_FALL);
-                    const float alpha = m_new == -INFINITY ? 0.f : k8_exp2(m[n] - m_new);
-                    m[n] = m_new;
-                    l[n] *= alpha;
+                        for (int n = 0; n < NT; ++n) sc[n][t][0] = sc[n][t][1] = sc[n][t][2] = sc[n][t][3] = 0.f;
+#pragma unroll
+                        for (int i = 0; i < CHUNKS; i += 2) {
+                            uint32_t a[4];
+                            if (i + 1 < CHUNKS) k8_ldmatrix(a, base + k8_at(k_key + t * 16, i + (mat >> 1), rows_shift, false));
+                            else k8_ldmatrix_x2(a, base + k8_at(k_key + t * 16, i, rows_shift, false));
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) k8_mma(sc[n][t], a, qf[n][i], qf[n][i + 1]);
+                        }
+                    }
+                    // scale bytes of this lane's keys: 2 g and 2 g + 1 (the other way round from g = 4 on), 16 further on the same; 0 where there
+                    // is no page
+                    uint32_t kb[4], vb[4];
+                    {
+                        const uint8_t* bytes = scales + st * SCALE_BYTES;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const uint32_t k2 = *reinterpret_cast<const uint16_t*>(bytes + half * 32 + t * 16 + 2 * g);
+                            const uint32_t v2 = *reinterpret_cast<const uint16_t*>(bytes + TILE + half * 32 + t * 16 + 2 * g);
+                            const uint32_t k0 = k2 & 0xffu, k1 = k2 >> 8, v0 = v2 & 0xffu, v1 = v2 >> 8;
+                            kb[2 * t] = g >= 4 ? k1 : k0;
+                            kb[2 * t + 1] = g >= 4 ? k0 : k1;
+                            vb[2 * t] = g >= 4 ? v1 : v0;
+                            vb[2 * t + 1] = g >= 4 ? v0 : v1;
+                        }
+                    }
+                    const int key0 = (first / TILE + tile) * TILE + half * 32;
+                    const bool inside = key0 >= first && key0 + 31 <= last;
+                    const bool every = __all_sync(0xffffffffu, inside && kb[0] && kb[1] && kb[2] && kb[3]);
+                    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+                    if (!every) {
+                        // keys before the first, behind the last, or without a page do not count, and what lies in the place of their values
+                        // must not meet a weight of zero: it may be NaN.  (keep0, keep1: a byte to a key of the second product's
+                        // operand in this lane)
+                        uint32_t keep = 0u;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int kpos = key0 - half * 32 + (i & 1 ? my_b : my_a) + (i >> 1) * 16;
+                            if (kpos < first || kpos > last) kb[i] = 0u;
+                            if (!kb[i]) vb[i] = 0u;
+                            keep |= kb[i] ? 0xffu << (8 * i) : 0u;
+                        }
+                        keep0 = __shfl_sync(0xffffffffu, keep, 4 * c);
+                        keep1 = __shfl_sync(0xffffffffu, keep, 4 * c + 16);
+                    }
+                    uint32_t b0[NT], b1[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float t[4], mx = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float* q2 = sc[n][i >> 1] + 2 * (i & 1);
+                            t[i] = fmaf(q2[1], 0.0625f, q2[0]) * (rowfac[n] * kv8_scale(kb[i]));
+                            t[i] = kb[i] ? t[i] : -INFINITY;
+                            mx = fmaxf(mx, t[i] + ((float)vb[i] - 127.f));
+                        }
+                        // (heads, four of them, with a key that is near the reference from below)
+                        uint32_t near = __ballot_sync(0xffffffffu, mx >= m[n] - K8D_NEAR);
+                        near |= near >> 16;
+                        near |= near >> 8;
+                        near |= near >> 4;
+                        if (__any_sync(0xffffffffu, mx > m[n]) || (near & 0xfu) != 0xfu) {
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                            top[n] = fmaxf(top[n], mx);
+                            float m_new = fmaxf(m[n], mx);
+                            if (mx < m[n] - K8D_NEAR && mx > -INFINITY) m_new = fmaxf(mx, top[n] - K8D_FALL);
+                            const float alpha = m_new == -INFINITY ? 0.f : k8_exp2(m[n] - m_new);
+                            m[n] = m_new;
+                            l[n] *= alpha;
+#pragma unroll
+                            for (int i = 0; i < CHUNKS; ++i) {
+                                o[n][i][0] *= alpha; o[n][i][1] *= alpha; o[n][i][2] *= alpha; o[n][i][3] *= alpha;
+                            }
+                        }
+                        const float m_use = m[n] == -INFINITY ? 0.f : m[n];
+                        float wt[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float e = k8_exp2(t[i] - m_use);
+                            l[n] += e;
+                            wt[i] = e * kv8_scale(vb[i] + 8u);     // 2^8 times the weight
+                        }
+                        uint32_t hi4, lo4;
+                        k8_split(wt[0], wt[1], wt[2], wt[3], hi4, lo4);
+                        const int from = 4 * c + (g >> 1);
+                        const uint32_t h0 = __shfl_sync(0xffffffffu, hi4, from), l0 = __shfl_sync(0xffffffffu, lo4, from);
+                        const uint32_t h1 = __shfl_sync(0xffffffffu, hi4, from + 16), l1 = __shfl_sync(0xffffffffu, lo4, from + 16);
+                        b0[n] = g & 1 ? l0 : h0;
+                        b1[n] = g & 1 ? l1 : h1;
+                    }
 #pragma unroll
                     for (int i = 0; i < CHUNKS; ++i) {
-                        o[n][i][0] *= alpha; o[n][i][1] *= alpha; o[n][i][2] *= alpha; o[n][i][3] *= alpha;
+                        uint32_t r[4], a[4];
+                        k8_ldmatrix_trans(r, base + k8_at(v_key, i, rows_shift, true));
+                        a[0] = __byte_perm(r[0], r[1], 0x6420);
+                        a[1] = __byte_perm(r[0], r[1], 0x7531);
+                        a[2] = __byte_perm(r[2], r[3], 0x6420);
+                        a[3] = __byte_perm(r[2], r[3], 0x7531);
+                        if (!every) {
+                            a[0] &= keep0; a[1] &= keep0;
+                            a[2] &= keep1; a[3] &= keep1;
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) k8_mma(o[n][i], a, b0[n], b1[n]);
+                    }
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&empty[st]);
+                }
+                // ---- the pair's part is done: hand the sums over ----
+                if (ok && k > 0 && !__all_sync(0xffffffffu, tc::mbar_wait(&taken, (uint32_t)((k - 1) & 1)))) {
+                    give_up();
+                    ok = false;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    l[n] += __shfl_xor_sync(0xffffffffu, l[n], 4);
+                    l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
+                    l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
+                    float* to = merge + (warp * 4 * NT + 4 * n + c) * XROW;
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; ++i)
+                        *reinterpret_cast<float2*>(to + i * 16 + 2 * g) = make_float2(fmaf(o[n][i][1], 0.0625f, o[n][i][0]) * 0x1p-8f,
+                                                                                      fmaf(o[n][i][3], 0.0625f, o[n][i][2]) * 0x1p-8f);
+                    if (g == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m[n], l[n]);
+                }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&dumped);
+                if (!CL && (item0 < lo || item1 > hi)) {
+                    const int nparts = work.cta_of(item1 - 1) - work.cta_of(item0) + 1;
+                    if (nparts > K8D_FEW_PARTS) {
+                        late0 = n_late ? late0 : item0;
+                        late1 = item0;
+                        parts0 = n_late ? parts0 : nparts;
+                        parts1 = nparts;
+                        ++n_late;
                     }
                 }
-                const float m_use = m[n] == -INFINITY ? 0.f : m[n];
-                float wt[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e = k8_exp2(t[i] - m_use);
-                    l[n] += e;
-                    wt[i] = e * kv8_scale(vb[i] + 8u);     // 2^8 times the weight
-                }
-                uint32_t hi4, lo4;
-                k8_split(wt[0], wt[1], wt[2], wt[3], hi4, lo4);
-                const int from = 4 * c + (g >> 1);
-                const uint32_t h0 = __shfl_sync(0xffffffffu, hi4, from), l0 = __shfl_sync(0xffffffffu, lo4, from);
-                const uint32_t h1 = __shfl_sync(0xffffffffu, hi4, from + 16), l1 = __shfl_sync(0xffffffffu, lo4, from + 16);
-                b0[n] = g & 1 ? l0 : h0;
-                b1[n] = g & 1 ? l1 : h1;
+                at.tile = at.end - 1;
+                work.next(at, 1);
             }
-#pragma unroll
-            for (int i = 0; i < CHUNKS; ++i) {
-                uint32_t r[4], a[4];
-                k8_ldmatrix_trans(r, base + k8_at(v_key, i, rows_shift, true));
-                a[0] = __byte_perm(r[0], r[1], 0x6420);
-                a[1] = __byte_perm(r[0], r[1], 0x7531);
-                a[2] = __byte_perm(r[2], r[3], 0x6420);
-                a[3] = __byte_perm(r[2], r[3], 0x7531);
-                if (!every) {
-                    a[0] &= keep0; a[1] &= keep0;
-                    a[2] &= keep1; a[3] &= keep1;
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) k8_mma(o[n][i], a, b0[n], b1[n]);
+        }
+        // pairs of many parts: where all are there, bring them, this warp every CWARPS-th
+        for (int i = 0; i < n_late; ++i) {
+            if (!ok || !__all_sync(0xffffffffu, tc::mbar_wait(&join[i], 0))) {
+                give_up();
+                return;
             }
+            const bool all = s_join[i] != 0;
+            const int nparts = i ? parts1 : parts0, i0 = work.cta_of(i ? late1 : late0);
+            if (!all) continue;
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(&taken, (uint32_t)((k - 1) & 1)))) {
+                give_up();
+                return;
+            }
+            ++k;
+            gather(nparts, [&](int i, int h, int d, float2& ml, float4& po) {
+                const float* row = p.parts + (((size_t)(i0 + i) * 2 + (i == 0 ? 1 : 0)) * p.heads + h) * XROW;
+                ml = __ldcg(reinterpret_cast<const float2*>(row + HD));
+                po = __ldcg(reinterpret_cast<const float4*>(row + d));
+            });
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&empty[st]);
+            if (lane == 0) tc::mbar_arrive(&dumped);
         }
-        // ---- the pair's part is done: hand the sums over ----
-        if (ok && k > 0 && !__all_sync(0xffffffffu, tc::mbar_wait(&taken, (uint32_t)((k - 1) & 1)))) {
-            give_up();
-            ok = false;
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 4);
-            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 8);
-            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
-            float* to = merge + (warp * 4 * NT + 4 * n + c) * XROW;
-#pragma unroll
-            for (int i = 0; i < CHUNKS; ++i)
-                *reinterpret_cast<float2*>(to + i * 16 + 2 * g) = make_float2(fmaf(o[n][i][1], 0.0625f, o[n][i][0]) * 0x1p-8f,
-                                                                              fmaf(o[n][i][3], 0.0625f, o[n][i][2]) * 0x1p-8f);
-            if (g == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m[n], l[n]);
-        }
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&dumped);
-        if (!CL && (item0 < lo || item1 > hi)) {
-            const int nparts = work.cta_of(item1 - 1) - work.cta_of(item0) + 1;
-            if (nparts > K8D_FEW_PARTS) {
-                late0 = n_late ? late0 : item0;
-                late1 = item0;
-                parts0 = n_late ? parts0 : nparts;
-                parts1 = nparts;
-                ++n_late;
-            }
-        }
-        at.tile = at.end - 1;
-        work.next(at, 1);
-    }
-    }
-    // pairs of many parts: where all are there, bring them, this warp every CWARPS-th
-    for (int i = 0; i < n_late; ++i) {
-        if (!ok || !__all_sync(0xffffffffu, tc::mbar_wait(&join[i], 0))) {
-            give_up();
-            return;
-        }
-        const bool all = s_join[i] != 0;
-        const int nparts = i ? parts1 : parts0, i0 = work.cta_of(i ? late1 : late0);
-        if (!all) continue;
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(&taken, (uint32_t)((k - 1) & 1)))) {
-            give_up();
-            return;
-        }
-        ++k;
-        gather(nparts, [&](int i, int h, int d, float2& ml, float4& po) {
-            const float* row = p.parts + (((size_t)(i0 + i) * 2 + (i == 0 ? 1 : 0)) * p.heads + h) * XROW;
-            ml = __ldcg(reinterpret_cast<const float2*>(row + HD));
-            po = __ldcg(reinterpret_cast<const float4*>(row + d));
-        });
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&dumped);
-    }
     }
     if (CL && G > 1) {
         tc::cluster_sync();                                // every CTA's part is in its shared memory
@@ -942,9 +942,10 @@ AP_EXPORT long long ap_attention_kv8_decode_scratch(int nh, int nkv, int ctas) {
     return 16LL * ctas + 8LL * ctas * k8d_heads(nh, nkv) * XROW;
 }
 
-// One launch for T rows.  cluster 0: `ctas` CTAs share the work whatever its lengths.  cluster 1, 2, 4, 8 or 16: so many CTAs to every pair of a
-// row and a KV head, which add up their parts through the cluster's shared memory (for few pairs; no scratch).  scratch: ap_attention_kv8_decode_scratch bytes, 16-byte aligned, of any contents but those of a call that runs at
-// the same time; nonce: another one for every call on the same scratch (a call may be run again, as from a graph, once it has ended).
+// One launch for T rows.  cluster 0: `ctas` CTAs share the work whatever its lengths.  cluster 1, 2, 4, 8 or 16: so many CTAs to every pair
+// of a row and a KV head, which add up their parts through the cluster's shared memory (for few pairs; no scratch).  scratch:
+// ap_attention_kv8_decode_scratch bytes, 16-byte aligned, of any contents but those of a call that runs at the same time; nonce: another one
+// for every call on the same scratch (a call may be run again, as from a graph, once it has ended).
 AP_EXPORT int ap_attention_kv8_decode(const void* q, void* out, const void* cache, long long num_pages, long long page_bytes,
                                       const int* block_table, int max_blocks, int nseq, const int* token_seq, const int* positions,
                                       int T, int nh, int nkv, int hd, int P, float scale, int window, int ctas, int cluster, void* scratch,

@@ -9,18 +9,19 @@
 // on the tensor cores while the other's softmax warps work (one row to a thread, P in bfloat16 over the S it came from, O scaled
 // down only when a row's maximum has grown by more than 2^8 over its reference).  Its loads are one box to half a tile.
 //
-// Widening first costs 6 bytes of traffic to a number, half of it in L2 where the keys fit there.  Widening inside the second kernel, every
-// tile in every CTA that reads it, was built and measured: four to six warps needed 3400 to 5100 cycles to a key tile, loading a box to
-// a page 4400, where the products and the softmax need 3700: 1470 us for 2048 rows behind 30000 keys (1.2 TFLOP), the two
-// kernels 1015; 17 rows behind 8191 keys 39 us, the two kernels 31.
+// Widening first costs 5 bytes of traffic to a number (one read, two written, two read again), the last four in L2 where the keys fit there.
+// Widening inside the second kernel, every tile in every CTA that reads it, was built and measured: four to six warps needed 3400 to 5100
+// cycles to a key tile, loading a box to a page 4400, where the products and the softmax need 3700: 1470 us for 2048 rows behind 30000 keys
+// (1.04 TFLOP), the two kernels 1005; 17 rows behind 8191 keys 39 us, the two kernels 29.
 //
 // A query tile without a second one beside it (few rows) walks two key tiles at once, each half of the CTA its own: 17 rows behind 32000
-// keys 80 us, one by one 104.  2048 rows behind 30000 keys run at 1.2 PFLOP/s, 0.73 of the measured peak of a dense bfloat16 product, bound by
-// the softmax (exponentials, and the scores' way through registers) beside the products; few rows by the way from one key tile
-// to the next (2 us for two of them), the widening (6 us of 31 behind 8191 keys, 31 of 80 behind 32000) and the slices' meeting (7).
+// keys 77 us, one by one 104.  2048 rows behind 30000 keys run at 1.04 PFLOP/s, 0.62 of the measured peak of a dense bfloat16 product:
+// the tensor pipe and the exponentials are each about half busy, taking turns on the same scores.  Few rows are bound by the way
+// from one key tile to the next (2 us for two of them), the widening (6 us of 29 behind 8191 keys, 31 of 77 behind 32000) and the
+// slices' meeting (7).
 //
 // Few rows leave most SMs idle: then the keys are cut into slices, a cluster of 2, 4 or 8 CTAs works on one set of rows, and the slices'
-// sums are added up through distributed shared memory, every CTA taking its share of the rows.  One launch, no scratch.
+// sums are added up through distributed shared memory, every CTA taking its share of the rows: no third launch, no scratch for them.
 //
 // Every wait is bounded; when one runs out a status word is raised and the results are void.
 //
@@ -734,9 +735,10 @@ AP_EXPORT long long ap_attention_kv8_tcgen05_scratch(long long tiles, int nkv) {
     return (tiles * nkv * (2 * 2 * BKV * HD + 4) + 15) / 16 * 16;
 }
 
-// q: [T][nh][HD]; query_tiles: 1 or 2 to a CTA; total_ctas: the sum over the sequences of ceil(rows / tokens of a CTA); nsplit: 1, 2, 4 or 8 key slices; scale > 0;
-// tiles: tiles of 128 keys that a sequence's rows see at most, from the first one that they see on (keys beyond them are not seen);
-// scratch: ap_attention_kv8_tcgen05_scratch(nseq * tiles, nkv) bytes of any contents, 16-byte aligned, of no call that runs at the same time.
+// q: [T][nh][HD]; query_tiles: 1 or 2 to a CTA; total_ctas: the sum over the sequences of ceil(rows / tokens of a CTA); nsplit: 1, 2, 4 or
+// 8 key slices; scale > 0; tiles: tiles of 128 keys that a sequence's rows see at most, from the first one that they see on (keys beyond
+// them are not seen); scratch: ap_attention_kv8_tcgen05_scratch(nseq * tiles, nkv) bytes of any contents, 16-byte aligned, of no call that runs
+// at the same time.
 AP_EXPORT int ap_attention_kv8_tcgen05(const void* q, void* out, const void* cache, long long num_pages, long long page_bytes,
                                        const int* block_table, int max_blocks, const int* seq_start, const int* positions, int nseq, int T,
                                        int nh, int nkv, int hd, int P, float scale, int window, int query_tiles, int total_ctas, int nsplit, int tiles, void* scratch,
