@@ -99,3 +99,39 @@ def test_a_key_that_a_page_given_back_held(ops):   # noqa: F811
     gone[c["table"][c["table"] >= 0].long()] = False
     c["pages"][gone] = 0x7f
     check(ops, c, 0, [(0, 899, 1, 3, 1), (1, 250, 0, None, 1)])
+
+
+@pytest.mark.parametrize("every", [1, 128])
+@pytest.mark.parametrize("window", [0, 1000])
+def test_a_long_portion_full_of_them(ops, every, window):   # noqa: F811
+    """Every value, or one column of every 128th key: a result for every row, in a bounded time."""
+    nh, nkv, hd, P, rows, keys = 8, 2, 128, 16, 2048, 10240
+    g = torch.Generator().manual_seed(1)
+    pages = keys // P
+    cache = torch.randint(0, 120, (pages, ops.kv8_page_bytes(nkv, P, hd)), generator=g, dtype=torch.uint8)
+    data, scale = plain.split(cache, nkv, P, hd)
+    scale.fill_(119)
+    if every == 1:
+        data[:, 1] = 0x7f
+    else:
+        data[::every // P, 1, :, 3, 77] = 0xff              # keys 3, 131, 259 ...
+    args = [t.cuda() for t in (cache, torch.arange(pages).int().view(1, -1), torch.zeros(rows, dtype=torch.int32),
+                               torch.arange(keys - rows, keys).int())]
+    q = torch.randn(rows, nh * hd, generator=g).bfloat16().cuda()
+    out = torch.zeros_like(q)
+    kw = dict(seq_start=torch.tensor([0, rows], dtype=torch.int32, device="cuda"), query_lens=[rows], contexts=[keys])
+    times = []
+    for _ in range(3):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        ops.attention_kv8(q, out, *args, nh, nkv, hd, P, 0.05, window, **kw)
+        end.record()
+        torch.cuda.synchronize()
+        times.append(start.elapsed_time(end))
+    ops.check_kernel_status()
+    nan = torch.isnan(out.view(rows, nh, hd)).cpu()
+    want = torch.ones_like(nan)
+    if every > 1:
+        want[:, :, :] = torch.arange(hd) == 77
+    assert torch.equal(nan, want)
+    assert min(times) < 100, times
